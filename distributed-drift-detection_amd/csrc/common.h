@@ -20,6 +20,15 @@ inline int launch_status(const char* where) { return hip_status(hipGetLastError(
 
 inline hipStream_t as_hip(ddm_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
+// launch() between the caller's timing events (either may be NULL).
+template <typename F>
+int timed(ddm_event_t begin, ddm_event_t end, hipStream_t s, F launch) {
+    if (begin)
+        if (int rc = hip_status(hipEventRecord(reinterpret_cast<hipEvent_t>(begin), s), "event record")) return rc;
+    if (int rc = launch()) return rc;
+    return end ? hip_status(hipEventRecord(reinterpret_cast<hipEvent_t>(end), s), "event record") : 0;
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A pointer into device (global) memory as the global address space: loads and stores

@@ -1,0 +1,208 @@
+// Rows of logits in registers: types, guarded wide loads, the running softmax of a lane and
+// the merges of its parts (token_scores.hip, distill.hip).
+#pragma once
+#include <float.h>
+
+#include "common.h"
+
+namespace ddm {
+namespace logits {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// exp2 of anything at or below this is 0 in float32; products e * d take d clamped here, so
+// that a masked entry (d = -inf, e = 0) adds 0 and not 0 * inf
+constexpr float kDead = -200.0f;
+
+struct f32_t {
+    static constexpr int kCode = DDM_F32, kSize = 4, kVec = 4;
+    static constexpr uint32_t kNegInf = 0xff800000u;     // one 32-bit word of -inf entries
+    static __device__ __forceinline__ float one(const char* p) { return *(const float*)p; }
+    static __device__ __forceinline__ uint32_t bits(const char* p) { return *(const uint32_t*)p; }
+    static __device__ __forceinline__ void store(char* p, float v) { *(float*)p = v; }
+};
+struct bf16_t {
+    static constexpr int kCode = DDM_BF16, kSize = 2, kVec = 8;
+    static constexpr uint32_t kNegInf = 0xff80ff80u;
+    static __device__ __forceinline__ float one(const char* p) {
+        return __uint_as_float((uint32_t)*(const uint16_t*)p << 16);
+    }
+    static __device__ __forceinline__ uint32_t bits(const char* p) { return *(const uint16_t*)p; }
+    static __device__ __forceinline__ void store(char* p, float v) { *(__bf16*)p = (__bf16)v; }
+};
+struct f16_t {
+    static constexpr int kCode = DDM_F16, kSize = 2, kVec = 8;
+    static constexpr uint32_t kNegInf = 0xfc00fc00u;
+    static __device__ __forceinline__ float one(const char* p) { return (float)*(const _Float16*)p; }
+    static __device__ __forceinline__ uint32_t bits(const char* p) { return *(const uint16_t*)p; }
+    static __device__ __forceinline__ void store(char* p, float v) { *(_Float16*)p = (_Float16)v; }
+};
+
+// 16 bytes of entries as float32.
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[4], f32_t) {
+    f[0] = __uint_as_float(r.x);
+    f[1] = __uint_as_float(r.y);
+    f[2] = __uint_as_float(r.z);
+    f[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[8], bf16_t) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[8], f16_t) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h2 h;
+        __builtin_memcpy(&h, &w[i], 4);
+        f[2 * i] = (float)h.x;
+        f[2 * i + 1] = (float)h.y;
+    }
+}
+// ... and back, rounded to nearest even once.
+__device__ __forceinline__ uint4 pack(const float (&f)[4], f32_t) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+template <typename H>
+__device__ __forceinline__ uint4 pack_half(const float (&f)[8]) {
+    typedef H h2 __attribute__((ext_vector_type(2)));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const h2 h = {(H)f[2 * i], (H)f[2 * i + 1]};
+        __builtin_memcpy(&w[i], &h, 4);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], bf16_t) { return pack_half<__bf16>(f); }
+__device__ __forceinline__ uint4 pack(const float (&f)[8], f16_t) { return pack_half<_Float16>(f); }
+
+// A row as 16-byte aligned vectors: vector j holds the columns j*kVec - head + [0, kVec), of
+// which those outside [0, v) are no entries.  Rows of an odd length start at any entry, so
+// `head` differs from row to row; only vectors that lie wholly inside are loaded as one,
+// the two at the ends entry by entry, and nothing outside the row is touched.
+template <typename T>
+struct Row {
+    const char* base;    // address of column 0
+    int v;
+    int head;            // entries between the aligned address below base and base
+    __device__ __forceinline__ Row(const char* p, int64_t n) : base(p), v((int)n) {
+        head = (int)(((uintptr_t)p & 15) / T::kSize);
+    }
+    __device__ __forceinline__ int col(int j) const { return j * T::kVec - head; }
+    __device__ __forceinline__ int vector_of(int c) const { return (c + head) / T::kVec; }
+    __device__ __forceinline__ bool whole(int j) const { return col(j) >= 0 && col(j) + T::kVec <= v; }
+    __device__ __forceinline__ uint4 load_whole(int j) const { return *(const uint4*)(base + col(j) * T::kSize); }
+    __device__ __forceinline__ float at(int c) const { return T::one(base + c * T::kSize); }
+    __device__ __forceinline__ uint4 load(int j) const {
+        if (whole(j)) return load_whole(j);
+        uint32_t w[4] = {T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+        const int c0 = col(j);
+        if (c0 < v) {
+#pragma unroll
+            for (int e = 0; e < T::kVec; ++e) {
+                const int c = c0 + e;
+                if (c >= 0 && c < v) {
+                    const uint32_t b = T::bits(base + c * T::kSize);
+                    if (T::kSize == 4)
+                        w[e & 3] = b;
+                    else
+                        w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xffffu) | (b << 16) : (w[e >> 1] & 0xffff0000u) | b;
+                }
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // The vector's entries into another row (gradients), as one where that is aligned alike.
+    __device__ __forceinline__ void store(char* out, int j, const float (&f)[T::kVec]) const {
+        const int c0 = col(j);
+        char* p = out + c0 * T::kSize;
+        if (whole(j) && ((uintptr_t)p & 15) == 0) {
+            *(uint4*)p = pack(f, T());
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < T::kVec; ++e)
+            if (c0 + e >= 0 && c0 + e < v) T::store(p + e * T::kSize, f[e]);
+    }
+};
+
+// NV vectors a lane of the part of a row that starts at vector j0 (lane stride: NT vectors,
+// so a wave's load covers 1 KB without a gap).  Parts without a row's end in them take the
+// branch with plain loads.
+template <typename T, int NT, int NV>
+__device__ __forceinline__ void load_part(const Row<T>& row, int j0, uint4 (&raw)[NV]) {
+    if (row.whole(j0) && row.whole(j0 + NT * NV - 1)) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = row.load_whole(j0 + i * NT + (int)threadIdx.x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = row.load(j0 + i * NT + (int)threadIdx.x);
+    }
+}
+
+// The same vector, but unknown to the compiler: what was computed from it before is not kept
+// in registers for a later pass (eight floats a vector), which unpacks it again.
+__device__ __forceinline__ uint4 again(uint4 r) {
+    asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
+    return r;
+}
+
+// A part's softmax: with d_i = (x_i - m) log2(e) / T over its entries, s = sum 2^d_i and
+// u = sum 2^d_i d_i.  m starts at the lowest finite value, so that -inf entries (d = -inf)
+// add nothing and a part of them alone has s = 0; NaN and +inf make s NaN for good.
+struct Part {
+    float m, s, u;
+};
+__device__ __forceinline__ Part no_part() { return Part{-FLT_MAX, 0.0f, 0.0f}; }
+
+__device__ __forceinline__ void rebase(Part& a, float m, float c) {
+    const float d = fmaxf((a.m - m) * c, kDead), r = __builtin_amdgcn_exp2f(d);
+    a.u = r * fmaf(a.s, d, a.u);
+    a.s *= r;
+    a.m = m;
+}
+__device__ __forceinline__ Part merge(Part a, Part b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    rebase(a, m, c);
+    rebase(b, m, c);
+    return Part{m, a.s + b.s, a.u + b.u};
+}
+__device__ __forceinline__ Part wave_merge(Part a, float c) {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) {
+        Part b;
+        b.m = __shfl_xor(a.m, k);
+        b.s = __shfl_xor(a.s, k);
+        b.u = __shfl_xor(a.u, k);
+        a = merge(a, b, c);
+    }
+    return a;
+}
+
+// float32 as an unsigned integer of the same order (-0 as +0); -inf is kKeyNegInf.
+constexpr uint32_t kKeyNegInf = 0x007fffffu;
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+// The next float32 below x (x finite).
+__device__ __forceinline__ float below(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return __uint_as_float(b == 0u ? 0x80000001u : (b >> 31) ? b + 1u : b - 1u);
+}
+
+__device__ __forceinline__ int64_t target_at(const void* t, int wide, int64_t i) {
+    return wide ? ((const int64_t*)t)[i] : (int64_t)((const int32_t*)t)[i];
+}
+
+}  // namespace logits
+}  // namespace ddm

@@ -1,0 +1,556 @@
+// What a language model answered, for the drift scans: log probability, entropy, rank, error
+// flag and the top alternatives of every row of logits, in one pass over them; and the
+// gradient of weighted log probabilities, entropies and alternatives.
+//
+// With d_i = (x_i - m) / T, m the row's maximum, S = sum e^d_i, U = sum e^d_i d_i:
+//   log p_i = d_i - log S,   H = log S - U / S,   rank = #{x_i > x_t or x_i = x_t, i < t}.
+// The pass is bound by reading the logits; what it computes per entry (about 13 vector
+// operations, one of them an exponential at a quarter of the rate) is just under what hides
+// behind that for 16-bit logits.  A row is cut into parts of at most kPartBytes, one a
+// workgroup, so that several workgroups share a CU and one's sums run behind another's loads;
+// few rows are cut finer, until there are enough workgroups for the chip.  Parts meet in a
+// second small launch.  No atomic decides an order: every sum is a fixed tree, and the
+// alternatives are ordered by (value, index).
+#include <type_traits>
+
+#include "logits.h"
+
+namespace ddm {
+namespace logits {
+
+constexpr int kMaxTop = 64;
+constexpr int kListCap = 512;        // candidates a selection keeps in LDS
+constexpr int kMaxParts = 64;        // parts of a row
+
+struct ScoreArgs {
+    const char* x;
+    int64_t n, v, ld_bytes;
+    const void* target;
+    int target_wide;
+    float temperature;
+    int top, parts;
+    float *logprob, *entropy, *stats, *top_logprob;
+    int32_t *rank, *top_index;
+    uint8_t* err;
+    float4* part_sum;        // [n][parts] m, s, u, rank count as bits
+    uint64_t* part_top;      // [n][parts][top] (key << 32) | ~column, 0: none
+};
+
+// ---- the k largest of a workgroup's entries ----------------------------------------------------
+// A lane's largest entry is a lower bound with a witness of its own, so the k-th largest of a
+// wave's 64 lane maxima bounds the k-th largest entry from below; the best of the waves'
+// bounds leaves little more than k candidates, which go to LDS and are ordered by counting.
+// More candidates than the list holds (rows of equal values) are cut exactly by bisection.
+struct SelectLds {
+    uint64_t list[kListCap];
+    uint32_t tau[16], n, sum[16];
+};
+
+// The k-th largest of the wave's keys (1 if fewer than k are above kKeyNegInf): bits from the
+// top, one ballot each; once exactly k remain, the prefix itself will do.
+__device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
+    uint32_t prefix = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t t = prefix | (1u << bit);
+        const int c = __popcll(__ballot(key >= t));
+        if (c >= k) {
+            prefix = t;
+            if (c == k) break;
+        }
+    }
+    return prefix > kKeyNegInf ? prefix : kKeyNegInf + 1;
+}
+
+template <int NT>
+__device__ __forceinline__ uint32_t block_sum(uint32_t v, SelectLds& l) {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k);
+    if (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) l.sum[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint32_t t = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) t += l.sum[w];
+    return t;
+}
+
+// each(fn): fn(key, column) for every entry of the lane; out(rank, packed) for rank 0..k-1.
+template <int NT, class Each, class Out>
+__device__ __forceinline__ void select_top(SelectLds& l, uint32_t lane_max, int k, Each each, Out out) {
+    uint32_t tau = wave_kth(lane_max, k);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) l.tau[threadIdx.x >> 6] = tau;
+    if (threadIdx.x == 0) l.n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) tau = max(tau, l.tau[w]);
+    if (lane_max >= tau)
+        each(tau, [&](uint32_t key, uint32_t col) {
+            const uint32_t at = atomicAdd(&l.n, 1u);
+            if (at < (uint32_t)kListCap) l.list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
+        });
+    __syncthreads();
+    uint32_t n = l.n;
+    if (n > (uint32_t)kListCap) {
+        // the k-th value exactly (32 halvings), then how far its ties reach (32 more)
+        uint32_t lo = tau, hi = 0xffffffffu;            // count(>= lo) >= k, and > hi holds none
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2 + 1;
+            uint32_t c = 0;
+            each(mid, [&](uint32_t, uint32_t) { ++c; });
+            if (block_sum<NT>(c, l) >= (uint32_t)k)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        const uint32_t kth = lo;
+        uint32_t more = 0;
+        each(kth, [&](uint32_t key, uint32_t) { more += key > kth; });
+        const uint32_t ties = (uint32_t)k - block_sum<NT>(more, l);
+        uint32_t a = 0, b = 0xffffffffu;                // the lowest column with `ties` ties up to it
+        while (a < b) {
+            const uint32_t mid = a + (b - a) / 2;
+            uint32_t c = 0;
+            each(kth, [&](uint32_t key, uint32_t col) { c += key == kth && col <= mid; });
+            if (block_sum<NT>(c, l) >= ties)
+                b = mid;
+            else
+                a = mid + 1;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) l.n = 0;
+        __syncthreads();
+        each(kth, [&](uint32_t key, uint32_t col) {
+            if (key > kth || col <= a) {
+                const uint32_t at = atomicAdd(&l.n, 1u);
+                if (at < (uint32_t)kListCap) l.list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
+            }
+        });
+        __syncthreads();
+        n = min(l.n, (uint32_t)kListCap);
+    }
+    for (uint32_t i = threadIdx.x; i < n; i += NT) {
+        const uint64_t me = l.list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += l.list[j] > me;
+        if (rank < (uint32_t)k) out((int)rank, me);
+    }
+    for (uint32_t i = n + threadIdx.x; i < (uint32_t)k; i += NT) out((int)i, 0ull);
+}
+
+// ---- one row's results -------------------------------------------------------------------------
+// What is common to a row: its maximum, log S (0 for a row with nothing left, NaN for a row
+// with NaN or +inf in it).
+struct RowLog {
+    float m, log_s;
+    bool bad, alive;
+};
+__device__ __forceinline__ RowLog row_log(const Part& p) {
+    RowLog r;
+    r.m = p.m;
+    r.bad = p.s != p.s;
+    r.alive = p.s > 0.0f;
+    r.log_s = r.alive ? __builtin_amdgcn_logf(p.s) * kLn2 : 0.0f;
+    return r;
+}
+
+// One thread writes the row's numbers; `ahead` counts the entries before the target's place.
+template <typename T>
+__device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t r, const Part& p, uint32_t ahead) {
+    const RowLog g = row_log(p);
+    const float nan = __builtin_nanf("");
+    const int64_t t = target_at(a.target, a.target_wide, r);
+    const bool counts = t >= 0 && t < a.v;
+    float lp = 0.0f;
+    int32_t rank = -1;
+    uint8_t err = 0;
+    if (counts && g.bad) {
+        lp = nan;
+        err = 1;
+    } else if (counts) {
+        const float xt = T::one(a.x + r * a.ld_bytes + t * T::kSize);
+        lp = xt > -INFINITY ? (xt - g.m) / a.temperature - g.log_s : xt;
+        rank = (int32_t)(ahead + (xt > -INFINITY ? 0u : (uint32_t)t));
+        err = rank > 0 || !(xt > -INFINITY);
+    }
+    a.logprob[r] = lp;
+    a.entropy[r] = g.bad ? nan : g.alive ? fmaxf(g.log_s - p.u / p.s * kLn2, 0.0f) : 0.0f;
+    a.rank[r] = rank;
+    a.err[r] = err;
+    a.stats[2 * r] = g.m;
+    a.stats[2 * r + 1] = g.bad ? nan : g.alive ? __builtin_amdgcn_logf(p.s) : -INFINITY;
+    if (r == a.n - 1)                                  // the scans read whole 16-byte words
+        for (int64_t i = a.n; i < (a.n + 15) / 16 * 16; ++i) a.err[i] = 0;
+}
+
+__device__ __forceinline__ void write_top(const ScoreArgs& a, int64_t r, const RowLog& g, int k, uint64_t packed) {
+    const bool some = packed != 0 && !g.bad;
+    const float x = of_key((uint32_t)(packed >> 32));
+    a.top_index[r * a.top + k] = some ? (int32_t)~(uint32_t)packed : -1;
+    a.top_logprob[r * a.top + k] =
+        g.bad ? __builtin_nanf("") : some ? (x - g.m) / a.temperature - g.log_s : -INFINITY;
+}
+
+// ---- a part of a row ---------------------------------------------------------------------------
+template <typename T, int NT, int NV, bool TOP>
+__global__ __launch_bounds__(NT) void k_score_parts(ScoreArgs a) {
+    constexpr int W = NT / 64;
+    __shared__ SelectLds sel;
+    __shared__ Part sh_part[W];
+    __shared__ uint32_t sh_ahead[W];
+    const int64_t r = blockIdx.x / a.parts;
+    const int part = (int)(blockIdx.x % a.parts);
+    const Row<T> row(a.x + r * a.ld_bytes, a.v);
+    const int j0 = part * NT * NV;
+    uint4 raw[NV];
+    load_part<T, NT, NV>(row, j0, raw);
+
+    const float c = kLog2e / a.temperature;
+    const int64_t t = target_at(a.target, a.target_wide, r);
+    const bool counts = t >= 0 && t < a.v;
+    const int t32 = counts ? (int)t : -1;
+    const float xt = counts ? row.at((int)t) : 0.0f;
+    // entries before the target's column are ahead of it at equal value; a masked target has
+    // every column before it ahead (added with the row) and the alive ones after it
+    const float thr_after = counts ? xt : INFINITY;
+    const float thr_before = counts && xt > -INFINITY ? below(xt) : INFINITY;
+
+    Part p = no_part();
+    float best[NV];
+    uint32_t ahead = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[T::kVec];
+        unpack(raw[i], f, T());
+        float m = f[0];
+#pragma unroll
+        for (int e = 1; e < T::kVec; ++e) m = fmaxf(m, f[e]);
+        best[i] = m;
+        if (__any(m > p.m)) rebase(p, fmaxf(p.m, m), c);
+        const float thr = row.col(j0 + i * NT + (int)threadIdx.x) + (T::kVec - 1) < t32 ? thr_before : thr_after;
+#pragma unroll
+        for (int e = 0; e < T::kVec; ++e) {
+            const float d = (f[e] - p.m) * c;
+            const float w = __builtin_amdgcn_exp2f(d);
+            p.s += w;
+            p.u = fmaf(w, fmaxf(d, kDead), p.u);
+            ahead += (uint32_t)__popcll(__ballot(f[e] > thr));
+        }
+    }
+    float lane_best = best[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) lane_best = fmaxf(lane_best, best[i]);
+    p = wave_merge(p, c);
+    if (W > 1) {
+        if ((threadIdx.x & 63) == 0) {
+            sh_part[threadIdx.x >> 6] = p;
+            sh_ahead[threadIdx.x >> 6] = ahead;
+        }
+        __syncthreads();
+        p = sh_part[0];
+        ahead = sh_ahead[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            p = merge(p, sh_part[w], c);
+            ahead += sh_ahead[w];
+        }
+    }
+    if (threadIdx.x == 0) {
+        if (counts) {                                  // the entries before it in its own vector
+            const int jt = row.vector_of(t32);
+            if (jt >= j0 && jt < j0 + NT * NV)
+                for (int i = max(row.col(jt), 0); i < t32; ++i)
+                    ahead += xt > -INFINITY ? (uint32_t)(row.at(i) == xt) : -(uint32_t)(row.at(i) > xt);
+        }
+        if (a.parts == 1)
+            write_row<T>(a, r, p, ahead);
+        else
+            a.part_sum[r * a.parts + part] = make_float4(p.m, p.s, p.u, __uint_as_float(ahead));
+    }
+    if (!TOP) return;
+    const RowLog g = row_log(p);
+    select_top<NT>(
+        sel, key_of(lane_best), a.top,
+        [&](uint32_t tau, auto fn) {
+            const float at_least = of_key(tau);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (best[i] >= at_least) {
+                    float f[T::kVec];
+                    unpack(again(raw[i]), f, T());
+                    const int c0 = row.col(j0 + i * NT + (int)threadIdx.x);
+#pragma unroll
+                    for (int e = 0; e < T::kVec; ++e)
+                        if (f[e] >= at_least) fn(key_of(f[e]), (uint32_t)(c0 + e));
+                }
+            }
+        },
+        [&](int k, uint64_t packed) {
+            if (a.parts == 1)
+                write_top(a, r, g, k, packed);
+            else
+                a.part_top[(r * a.parts + part) * a.top + k] = packed;
+        });
+}
+
+// ---- the parts of a row joined -------------------------------------------------------------------
+template <typename T, bool TOP>
+__global__ __launch_bounds__(TOP ? 256 : 64) void k_score_join(ScoreArgs a) {
+    constexpr int NT = TOP ? 256 : 64, NC = kMaxParts * kMaxTop / NT;
+    __shared__ SelectLds sel;
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    const float c = kLog2e / a.temperature;
+    Part p = no_part();
+    uint32_t ahead = 0;
+    if (lane < a.parts) {                              // every wave for itself
+        const float4 q = a.part_sum[r * a.parts + lane];
+        p = Part{q.x, q.y, q.z};
+        ahead = __float_as_uint(q.w);
+    }
+    p = wave_merge(p, c);
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) ahead += __shfl_xor(ahead, k);
+    if (threadIdx.x == 0) write_row<T>(a, r, p, ahead);
+    if (!TOP) return;
+    const RowLog g = row_log(p);
+    const int n = a.parts * a.top;
+    const uint64_t* from = a.part_top + r * n;
+    uint64_t cand[NC];
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int at = i * NT + (int)threadIdx.x;
+        cand[i] = at < n ? from[at] : 0;
+        best = max(best, (uint32_t)(cand[i] >> 32));
+    }
+    select_top<NT>(
+        sel, best, a.top,
+        [&](uint32_t tau, auto fn) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if ((uint32_t)(cand[i] >> 32) >= tau) fn((uint32_t)(cand[i] >> 32), ~(uint32_t)cand[i]);
+        },
+        [&](int k, uint64_t packed) { write_top(a, r, g, k, packed); });
+}
+
+// ---- gradient ------------------------------------------------------------------------------------
+// dx_i = (-p_i (A + B log p_i) + [i = t] g_lp + [i = index_k] g_top,k) / T with
+// A = g_lp + sum g_top + g_H H, B = g_H: elementwise from the forward's statistics, reading and
+// writing every logit once.  The few columns with a term of their own are written again after
+// the rest of their part, in full, by one lane each.
+struct GradArgs {
+    const char* x;
+    int64_t n, v, ld_bytes, out_ld_bytes;
+    const void* target;
+    int target_wide;
+    float temperature;
+    int top, parts;
+    const float *stats, *entropy;
+    const int32_t* top_index;
+    const float *d_logprob, *d_entropy, *d_top;
+    char* out;
+};
+
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT) void k_score_grad(GradArgs a) {
+    const int64_t r = blockIdx.x / a.parts;
+    const int part = (int)(blockIdx.x % a.parts);
+    const Row<T> row(a.x + r * a.ld_bytes, a.v);
+    char* out = a.out + r * a.out_ld_bytes;
+    const int j0 = part * NT * NV;
+    uint4 raw[NV];
+    load_part<T, NT, NV>(row, j0, raw);
+    const int lane = threadIdx.x & 63;
+    const float m = a.stats[2 * r], log2_s = a.stats[2 * r + 1];
+    const float c = kLog2e / a.temperature, inv_t = 1.0f / a.temperature;
+    const int64_t t = target_at(a.target, a.target_wide, r);
+    const bool counts = t >= 0 && t < a.v;
+    const float g_lp = counts && a.d_logprob ? a.d_logprob[r] : 0.0f;
+    const float g_h = a.d_entropy ? a.d_entropy[r] : 0.0f;
+    int32_t index = -1;
+    float g_top = 0.0f;
+    if (lane < a.top) {
+        index = a.top_index[r * a.top + lane];
+        if (index >= 0) g_top = a.d_top[r * a.top + lane];
+    }
+    float all_top = g_top;
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) all_top += __shfl_xor(all_top, k);
+    const float A = -(g_lp + all_top + g_h * a.entropy[r]) * inv_t, B = -g_h * kLn2 * inv_t;
+    const bool dead = log2_s == -INFINITY;              // nothing left: no gradient
+    // the columns with a term of their own, read before any store: out may be the logits
+    auto mine = [&](int col) {
+        const int j = row.vector_of(col);
+        return j >= j0 && j < j0 + NT * NV;
+    };
+    const bool first = threadIdx.x < 64;
+    const bool put_top = first && index >= 0 && mine(index);
+    const bool put_t = threadIdx.x == 0 && counts && mine((int)t);
+    const float x_top = put_top ? row.at(index) : 0.0f, x_t = put_t ? row.at((int)t) : 0.0f;
+    __syncthreads();
+    auto value = [&](float x) {
+        const float d = (x - m) * c - log2_s;
+        return dead ? 0.0f : __builtin_amdgcn_exp2f(d) * fmaf(B, fmaxf(d, kDead), A);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[T::kVec];
+        unpack(raw[i], f, T());
+#pragma unroll
+        for (int e = 0; e < T::kVec; ++e) f[e] = value(f[e]);
+        row.store(out, j0 + i * NT + (int)threadIdx.x, f);
+    }
+    __syncthreads();
+    auto put = [&](int col, float x, float extra) {
+        T::store(out + col * T::kSize, dead ? 0.0f : fmaf(extra, inv_t, value(x)));
+    };
+    const bool listed = __any(counts && index == t);
+    if (put_top) put(index, x_top, g_top + (counts && index == t ? g_lp : 0.0f));
+    if (put_t && !listed) put((int)t, x_t, g_lp);
+}
+
+// ---- launch shapes ---------------------------------------------------------------------------------
+// One wave a row while the row fits its registers (512 vectors of 16 bytes); longer rows in
+// parts of 256 lanes, 8 vectors each, or fewer while there are not workgroups enough to fill
+// 256 CUs several times over.
+struct Shape {
+    int nt, nv, parts;
+};
+inline Shape shape_of(int64_t n, int64_t v, int vec) {
+    const int64_t nvec = ceil_div(v + vec - 1, vec);     // whatever the rows' alignment
+    Shape s;
+    if (nvec <= 64 * 8) {
+        s.nt = 64;
+        s.nv = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
+    } else {
+        s.nt = 256;
+        s.nv = 8;
+        while (s.nv > 1 && n * ceil_div(nvec, 256 * s.nv) < 1024 && ceil_div(nvec, 128 * s.nv) <= kMaxParts) s.nv /= 2;
+    }
+    s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv);
+    return s;
+}
+
+constexpr int64_t kMaxColumns = 1 << 19;
+
+template <typename F>
+int with_type(int32_t dtype, F f) {
+    switch (dtype) {
+        case DDM_F32: return f(f32_t());
+        case DDM_BF16: return f(bf16_t());
+        case DDM_F16: return f(f16_t());
+    }
+    return DDM_E_ARG;
+}
+template <typename F>
+void with_shape(const Shape& s, F f) {
+#define DDM_SHAPE(NT_, NV_) \
+    if (s.nt == NT_ && s.nv == NV_) return f(std::integral_constant<int, NT_>(), std::integral_constant<int, NV_>())
+    DDM_SHAPE(64, 1);
+    DDM_SHAPE(64, 2);
+    DDM_SHAPE(64, 4);
+    DDM_SHAPE(64, 8);
+    DDM_SHAPE(256, 1);
+    DDM_SHAPE(256, 2);
+    DDM_SHAPE(256, 4);
+    DDM_SHAPE(256, 8);
+#undef DDM_SHAPE
+}
+
+// The checks both entry points share; 0 or DDM_E_ARG with the reason.
+inline int check_rows(const char* who, int32_t dtype, int64_t n, int64_t v, int64_t ld, int32_t target_bytes,
+                      float temperature, int32_t top) {
+    if (dtype != DDM_F32 && dtype != DDM_BF16 && dtype != DDM_F16) {
+        set_error("%s: unknown type %d", who, (int)dtype);
+    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts) {
+        set_error("%s: invalid argument (rows %lld, columns %lld of 1..%lld, row stride %lld)", who, (long long)n,
+                  (long long)v, (long long)kMaxColumns, (long long)ld);
+    } else if (target_bytes != 4 && target_bytes != 8) {
+        set_error("%s: targets of %d bytes (4 or 8)", who, (int)target_bytes);
+    } else if (!(temperature > 0.0f) || !(temperature < INFINITY)) {
+        set_error("%s: temperature must be positive and finite", who);
+    } else if (top < 0 || top > kMaxTop) {
+        set_error("%s: %d alternatives (0..%d)", who, (int)top, kMaxTop);
+    } else {
+        return 0;
+    }
+    return DDM_E_ARG;
+}
+
+}  // namespace logits
+}  // namespace ddm
+
+using namespace ddm;
+using namespace ddm::logits;
+
+extern "C" int64_t ddm_token_scores_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t top) {
+    if (n <= 0 || v < 1 || v > kMaxColumns || top < 0 || top > kMaxTop) return 0;
+    const Shape s = shape_of(n, v, dtype == DDM_F32 ? 4 : 8);
+    return s.parts == 1 ? 0 : n * s.parts * (16 + 8 * (int64_t)top);
+}
+
+extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld,
+                                const void* target, int32_t target_bytes, float temperature, int32_t top,
+                                float* logprob, float* entropy, float* stats, int32_t* rank, uint8_t* err,
+                                float* top_logprob, int32_t* top_index, void* scratch, ddm_stream_t stream,
+                                ddm_event_t ev_begin, ddm_event_t ev_end) {
+    if (int rc = check_rows("ddm_token_scores", dtype, n, v, ld, target_bytes, temperature, top)) return rc;
+    if (n == 0) return 0;
+    const Shape s = shape_of(n, v, dtype == DDM_F32 ? 4 : 8);
+    if (!logits || !target || !logprob || !entropy || !stats || !rank || !err || (top && (!top_logprob || !top_index)) ||
+        (s.parts > 1 && !scratch)) {
+        set_error("ddm_token_scores: invalid argument (null pointer)");
+        return DDM_E_ARG;
+    }
+    const hipStream_t st = as_hip(stream);
+    return timed(ev_begin, ev_end, st, [&] {
+        return with_type(dtype, [&](auto type) {
+            using T = decltype(type);
+            ScoreArgs a{(const char*)logits, n, v, ld * T::kSize, target, target_bytes == 8, temperature, top, s.parts,
+                        logprob, entropy, stats, top_logprob, rank, top_index, err, (float4*)scratch,
+                        (uint64_t*)((char*)scratch + n * s.parts * 16)};
+            with_shape(s, [&](auto nt, auto nv) {
+                if (top)
+                    k_score_parts<T, nt(), nv(), true><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
+                else
+                    k_score_parts<T, nt(), nv(), false><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
+            });
+            if (int rc = launch_status("ddm_token_scores")) return rc;
+            if (s.parts > 1) {
+                if (top)
+                    k_score_join<T, true><<<dim3((unsigned)n), 256, 0, st>>>(a);
+                else
+                    k_score_join<T, false><<<dim3((unsigned)n), 64, 0, st>>>(a);
+            }
+            return launch_status("ddm_token_scores");
+        });
+    });
+}
+
+extern "C" int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld,
+                                     const void* target, int32_t target_bytes, float temperature, int32_t top,
+                                     const float* stats, const float* entropy, const int32_t* top_index,
+                                     const float* d_logprob, const float* d_entropy, const float* d_top, void* out,
+                                     int64_t out_ld, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end) {
+    if (int rc = check_rows("ddm_token_scores_grad", dtype, n, v, ld, target_bytes, temperature, top)) return rc;
+    if (n == 0) return 0;
+    if (!logits || !target || !stats || !entropy || !out || out_ld < v || (top && (!top_index || !d_top))) {
+        set_error("ddm_token_scores_grad: invalid argument (null pointer or output stride)");
+        return DDM_E_ARG;
+    }
+    const Shape s = shape_of(n, v, dtype == DDM_F32 ? 4 : 8);
+    const hipStream_t st = as_hip(stream);
+    return timed(ev_begin, ev_end, st, [&] {
+        return with_type(dtype, [&](auto type) {
+            using T = decltype(type);
+            GradArgs a{(const char*)logits, n, v, ld * T::kSize, out_ld * T::kSize, target, target_bytes == 8,
+                       temperature, top, s.parts, stats, entropy, top_index, d_logprob, d_entropy, d_top, (char*)out};
+            with_shape(s, [&](auto nt, auto nv) {
+                k_score_grad<T, nt(), nv()><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
+            });
+            return launch_status("ddm_token_scores_grad");
+        });
+    });
+}

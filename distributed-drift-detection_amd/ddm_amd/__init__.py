@@ -15,6 +15,7 @@ __version__ = "0.1.0"
 _EXPORTS = {
     "run_DDM_loop": "controller", "run_partition_frame": "controller", "DevicePartition": "controller",
     "PartitionRunner": "controller", "DDMSettings": "params", "OUTPUT_COLUMNS": "params", "SCHEMA": "params",
+    "token_scores": "tokens", "token_scores_grad": "tokens", "TokenScores": "tokens",
     "MTStream": "rng", "DdmError": "_capi", "lib": "_capi",
 }
 

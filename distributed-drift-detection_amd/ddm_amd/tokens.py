@@ -1,0 +1,190 @@
+"""A language model in the place of the forest: what its answers say, and what a refit trains it on.
+
+`token_scores` is predict_rf's part (DDM_Process.py:110-128) for rows of logits: per answer
+the error flag the DDM scans read (`kernels.scan_streams` and its relatives), and next to it
+log probability, entropy, rank and the top alternatives; `token_scores_grad` is its backward
+pass.  `topk_distill` is the loss (and gradient) of train_rf's part (:98-105): a model
+refitted on the alternatives another one gave.
+
+The calls are asynchronous on `stream` (default: the current stream of the logits' device),
+read nothing back and can be captured.  Results belong to that stream.
+"""
+import collections
+import ctypes
+
+import torch
+
+from ._capi import check, lib
+from .kernels import _evs, _ptr
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_COLUMNS = 1 << 19
+MAX_TOP = 64
+
+TokenScores = collections.namedtuple("TokenScores", ["logprob", "entropy", "rank", "err", "top_logprob", "top_index",
+                                                     "stats", "temperature"])
+TokenScores.__doc__ = """What token_scores returns: logprob, entropy float32 [n]; rank int32 [n]; err uint8
+[n rounded up to 16] (the scans' layout, zeros behind row n-1); top_logprob float32 and top_index int32 [n, top]
+(None for top 0); stats float32 [n, 2] and the temperature, for token_scores_grad."""
+
+
+class launch_on:
+    """The device of `t` and the stream to launch on, as a context: what is allocated inside
+    belongs to that stream, and inputs stay alive for it."""
+
+    def __init__(self, t, stream, inputs):
+        if t.device.type != "cuda":
+            raise ValueError(f"tensors must be on the GPU, got {t.device}")
+        for x in inputs:
+            if x is not None and x.device != t.device:
+                raise ValueError(f"tensors on {t.device} and on {x.device}")
+        current = torch.cuda.current_stream(t.device)
+        self.stream = stream if stream is not None else current
+        if self.stream.device != t.device:
+            raise ValueError(f"stream of {self.stream.device}, tensors on {t.device}")
+        if self.stream != current:
+            for x in inputs:
+                if x is not None:
+                    x.record_stream(self.stream)
+        self.ctx = torch.cuda.stream(self.stream)
+
+    def __enter__(self):
+        self.ctx.__enter__()            # also makes the stream's device the current one
+        return ctypes.c_void_p(self.stream.cuda_stream)
+
+    def __exit__(self, *exc):
+        return self.ctx.__exit__(*exc)
+
+
+def rows_of(name, t, dtypes=DTYPES):
+    """The row stride of a matrix whose rows are contiguous."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has type {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}'s rows must be contiguous (strides {t.stride()})")
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise ValueError(f"{name}'s rows overlap (strides {t.stride()})")
+    return ld
+
+
+def shaped(name, t, shape, *dtypes):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} {list(shape)}, got {t.dtype} "
+                         f"{list(t.shape)}")
+
+
+def dense(t):
+    """`t` without gaps (a copy on the launch stream if it has any)."""
+    return None if t is None else t.contiguous()
+
+
+def _span(t):
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def overlap(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _temperature(t):
+    t = float(t)
+    if not 0.0 < t < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {t}")
+    return t
+
+
+def _logits(logits):
+    ld = rows_of("logits", logits)
+    n, v = logits.shape
+    if not 1 <= v <= MAX_COLUMNS:
+        raise ValueError(f"logits have {v} columns (1..{MAX_COLUMNS})")
+    return n, v, ld
+
+
+def _check_out(out, logits):
+    if out is None:
+        return
+    rows_of("out", out)
+    if out.shape != logits.shape or out.dtype != logits.dtype:
+        raise ValueError(f"out must be {logits.dtype} {list(logits.shape)}, got {out.dtype} {list(out.shape)}")
+    same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
+    if not same and overlap(out, logits):
+        raise ValueError("out overlaps the logits without being them")
+
+
+def _new_like(out, logits):
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+
+
+def token_scores(logits, targets, top=0, temperature=1.0, stream=None, timer=None):
+    """Scores of every row of logits [n, v] (float32, bfloat16 or float16; rows contiguous, any
+    row stride) against targets [n] (int32 or int64): see TokenScores.
+
+    A target outside [0, v) is not scored (logprob 0, rank -1, err 0).  -inf logits are masked:
+    probability 0, never an alternative; index -1 and -inf stand behind the last alternative.  A
+    row with nothing left has logprob -inf, entropy 0, err 1.  A row with NaN or +inf has NaN
+    scores, rank and indexes -1, err 1.  Equal logits rank by the lower column."""
+    n, v, ld = _logits(logits)
+    shaped("targets", targets, (n,), torch.int32, torch.int64)
+    top, temperature = int(top), _temperature(temperature)
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top must be 0..{MAX_TOP}, got {top}")
+    dev, code = logits.device, DTYPES[logits.dtype]
+    with launch_on(logits, stream, (logits, targets)) as s:
+        targets = dense(targets)
+        f32 = torch.empty((4, n), dtype=torch.float32, device=dev)
+        logprob, entropy, stats = f32[0], f32[1], f32[2:].view(-1)
+        rank = torch.empty(n, dtype=torch.int32, device=dev)
+        err = torch.empty((n + 15) // 16 * 16, dtype=torch.uint8, device=dev)
+        top_lp = torch.empty((n, top), dtype=torch.float32, device=dev) if top else None
+        top_ix = torch.empty((n, top), dtype=torch.int32, device=dev) if top else None
+        need = int(lib.ddm_token_scores_scratch_bytes(n, v, code, top))
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(lib.ddm_token_scores(logits.data_ptr(), code, n, v, ld, targets.data_ptr(), targets.element_size(),
+                                   temperature, top, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                   rank.data_ptr(), err.data_ptr(), _ptr(top_lp), _ptr(top_ix), _ptr(scratch), s,
+                                   *_evs(timer)), "ddm_token_scores")
+    return TokenScores(logprob, entropy, rank, err, top_lp, top_ix, stats.view(n, 2), temperature)
+
+
+def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d_top=None, out=None, stream=None,
+                      timer=None):
+    """Gradient by the logits of  d_logprob . logprob + d_entropy . entropy + d_top . top_logprob
+    (float32 [n], [n], [n, top]; None: zero), in the logits' type.  `scores` is what
+    token_scores returned for the same logits and targets.  out: None, the logits themselves
+    (overwritten), or a tensor of their shape apart from them."""
+    n, v, ld = _logits(logits)
+    shaped("targets", targets, (n,), torch.int32, torch.int64)
+    shaped("scores.stats", scores.stats, (n, 2), torch.float32)
+    shaped("scores.entropy", scores.entropy, (n,), torch.float32)
+    for name, g in (("d_logprob", d_logprob), ("d_entropy", d_entropy)):
+        if g is not None:
+            shaped(name, g, (n,), torch.float32)
+    top, index = 0, None
+    if d_top is not None:
+        if scores.top_index is None:
+            raise ValueError("d_top given, but the scores have no alternatives")
+        index, top = scores.top_index, scores.top_index.shape[1]
+        shaped("scores.top_index", index, (n, top), torch.int32)
+        shaped("d_top", d_top, (n, top), torch.float32)
+    _check_out(out, logits)
+    given = (logits, targets, scores.stats, scores.entropy, index, d_logprob, d_entropy, d_top, out)
+    with launch_on(logits, stream, given) as s:
+        targets, stats, entropy, index, d_logprob, d_entropy, d_top = map(dense, given[1:8])
+        out = _new_like(out, logits)
+        out_ld = out.stride(0) if n > 1 else v
+        check(lib.ddm_token_scores_grad(logits.data_ptr(), DTYPES[logits.dtype], n, v, ld, targets.data_ptr(),
+                                        targets.element_size(), scores.temperature, top, stats.data_ptr(),
+                                        entropy.data_ptr(), _ptr(index), _ptr(d_logprob), _ptr(d_entropy),
+                                        _ptr(d_top), out.data_ptr(), out_ld, s, *_evs(timer)),
+              "ddm_token_scores_grad")
+    return out

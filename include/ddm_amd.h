@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define DDM_AMD_ABI_VERSION 24
+#define DDM_AMD_ABI_VERSION 25
 
 #define DDM_E_ARG        1001   /* invalid argument (null pointer, bad size) */
 #define DDM_E_FOREST     1002   /* forest shape not supported (classes > 256) */
@@ -735,6 +735,42 @@ int ddm_ctl_graph_destroy(void* exec);
 int ddm_forest_predict_dev(const ddm_predict_segment* segs_dev, const int64_t* const* res_dev, int32_t n_segs,
                            int32_t per_batch, int64_t grid, int32_t* stall, ddm_stream_t stream,
                            ddm_event_t ev_begin, ddm_event_t ev_end);
+
+/* ---- language models: what is monitored, and what a refit trains on ----------------- */
+/* A language model's predictions are rows of logits.  ddm_token_scores is predict_rf for it
+ * (DDM_Process.py:110-128: the answers' error flags, :117), ddm_topk_distill the loss of its
+ * refit (:98-105), ddm_gated_scan the recurrence its scores' charts and its layers run on. */
+#define DDM_F32  0
+#define DDM_BF16 1
+#define DDM_F16  2
+
+/* Scores of n rows of v logits (v at most 524288; row stride ld >= v entries, any alignment)
+ * against target[n] (target_bytes 4: int32, 8: int64), at temperature T > 0:
+ *   logprob[n], entropy[n]   of softmax(x / T), float32
+ *   rank[n]    entries before the target in the order (value descending, column ascending)
+ *   err[ceil16(n)]  1: the target is not the first alternative (rank > 0, or masked), else 0;
+ *              the bytes behind row n - 1 are zeroed, so the scans can read whole words
+ *   stats[2n]  (maximum, log2 of the sum) for ddm_token_scores_grad
+ *   top_logprob[n * top], top_index[n * top]  the `top` (0..64) largest, in that order
+ * A target outside [0, v) is not scored: logprob 0, rank -1, err 0.  -inf entries are masked:
+ * never an alternative (index -1, logprob -inf behind the last), probability 0.  A row of them
+ * alone: logprob -inf, entropy 0, err 1, no alternatives, gradient 0.  A row with NaN or +inf:
+ * logprob, entropy, alternatives and gradient NaN, rank and index -1, err 1.
+ * scratch: ddm_token_scores_scratch_bytes(...) bytes, 16-byte aligned (NULL if 0). */
+int64_t ddm_token_scores_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t top);
+int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld, const void* target,
+                     int32_t target_bytes, float temperature, int32_t top, float* logprob, float* entropy,
+                     float* stats, int32_t* rank, uint8_t* err, float* top_logprob, int32_t* top_index,
+                     void* scratch, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
+/* Gradient of sum d_logprob logprob + d_entropy entropy + d_top top_logprob by the logits, in
+ * their type, to out (row stride out_ld): the logits' own buffer with their stride, or one
+ * that does not overlap it.  stats, entropy and top_index are the forward's;
+ * d_logprob and d_entropy may be NULL (0), top 0 leaves the alternatives out. */
+int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld, const void* target,
+                          int32_t target_bytes, float temperature, int32_t top, const float* stats,
+                          const float* entropy, const int32_t* top_index, const float* d_logprob,
+                          const float* d_entropy, const float* d_top, void* out, int64_t out_ld,
+                          ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
 
 /* ---- synthetic inputs (benchmark configs) ------------------------- */
 

@@ -1,0 +1,121 @@
+"""The language-model operators written out in float64 on the host, and what float32 costs them.
+
+U is half a step of float32.  A sum over a row is a chain of at most 64 additions in a lane and
+a tree of 18 over lanes, waves and parts (82 U), with at most 22 changes of the running maximum
+(an exponential of 2 U, a product of 1 U each, and arguments that telescope: 28 U), each term an
+exponential (2 U) of an argument with two roundings (1.4 U per nat of it, 18 U on average over a
+softmax of 2^19 columns): together under SUM = 200 half steps.
+"""
+import math
+
+import torch
+
+U = 2.0 ** -24
+SUM = 200
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def smallest(dtype):
+    """Half the spacing of the type's subnormal numbers."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def softmax64(x, temperature):
+    """log p, p of every row; a row with nothing left has log p = -inf, one with NaN or +inf has NaN."""
+    z = x.double() / temperature
+    dead = torch.isneginf(z).all(1, keepdim=True)
+    # by the maximum first: next to the type's lowest value even float64 has no room for log n
+    d = z - torch.where(dead, 0.0, z.amax(1, keepdim=True))
+    logp = d - torch.where(dead, 0.0, d.exp().sum(1, keepdim=True).log())
+    bad = (torch.isnan(z) | torch.isposinf(z)).any(1, keepdim=True)
+    return torch.where(bad, math.nan, logp), dead[:, 0], bad[:, 0]
+
+
+def scores64(x, t, top, temperature):
+    n, v = x.shape
+    logp, dead, bad = softmax64(x, temperature)
+    p = logp.exp()
+    counts = (t >= 0) & (t < v)
+    at = t.clamp(0, v - 1).long()[:, None]
+    xf = x.double()
+    xt = xf.gather(1, at)
+    before = torch.arange(v)[None, :] < at
+    ahead = ((xf > xt) | ((xf == xt) & before)).sum(1)
+    rank = torch.where(counts & ~bad, ahead, -1)
+    err = counts & (bad | (ahead > 0) | torch.isneginf(xt[:, 0]))
+    lp = torch.where(counts, logp.gather(1, at)[:, 0], 0.0)
+    entropy = torch.where(bad, math.nan, -torch.special.xlogy(p, p).sum(1))
+    out = {"logprob": lp, "entropy": entropy, "rank": rank.int(), "err": err.to(torch.uint8)}
+    if top:
+        # a stable sort of the negated values puts the lower column of equal ones first
+        k = min(top, v)
+        order = (-torch.where(torch.isnan(xf), -math.inf, xf)).sort(dim=1, stable=True).indices[:, :k]
+        value = logp.gather(1, order)
+        keep = ~torch.isneginf(xf.gather(1, order)) & ~bad[:, None]
+        value = torch.where(bad[:, None], math.nan, torch.where(keep, value, -math.inf))
+        index = torch.where(keep, order, -1)
+        pad = (0, top - k)
+        fill = torch.where(bad, math.nan, -math.inf)[:, None].expand(n, top - k)
+        out["top_logprob"] = torch.cat([value, fill], 1)
+        out["top_index"] = torch.nn.functional.pad(index, pad, value=-1).int()
+    return out
+
+
+def scores_tolerance(x, ref, temperature):
+    """Bounds on |logprob - exact| (also of the alternatives) and |entropy - exact|, float32."""
+    v = x.shape[1]
+    log_v = math.log(v) + 1.0
+    lp = lambda r: U * (SUM + 3 * log_v + 4 * torch.nan_to_num(r.abs(), posinf=0.0))  # noqa: E731
+    # H = log S - U/S: the first as above, the second a quotient of two sums of size <= log_v + H
+    h = U * (SUM + 3 * log_v + (2 * SUM + 10) * 2 * log_v)
+    return lp, h
+
+
+def scores_grad64(x, t, ref, temperature, d_logprob=None, d_entropy=None, d_top=None):
+    n, v = x.shape
+    logp, dead, bad = softmax64(x, temperature)
+    p = logp.exp()
+    counts = (t >= 0) & (t < v)
+    zero = torch.zeros(n, dtype=torch.float64)
+    g_lp = torch.where(counts, d_logprob.double(), 0.0) if d_logprob is not None else zero
+    g_h = d_entropy.double() if d_entropy is not None else zero
+    rows = torch.arange(n)
+    direct = torch.zeros(n, v, dtype=torch.float64)
+    direct[rows, t.clamp(0, v - 1).long()] += g_lp
+    a = g_lp.clone()
+    if d_top is not None:
+        listed = ref["top_index"] >= 0
+        g_top = torch.where(listed, d_top.double(), 0.0)
+        direct.scatter_add_(1, ref["top_index"].clamp(min=0).long(), g_top)
+        a = a + g_top.sum(1)
+    plogp = torch.special.xlogy(p, p)
+    dx = (direct - a[:, None] * p - g_h[:, None] * (plogp + p * ref["entropy"][:, None])) / temperature
+    dx = torch.where(bad[:, None], math.nan, torch.where(dead[:, None], 0.0, dx))
+    # float32: p to SUM + 8 per nat of its logarithm, the bracket to a few half steps of its parts
+    size = p * (a.abs()[:, None] + g_h.abs()[:, None] * (torch.nan_to_num(ref["entropy"].abs())[:, None] + 1))
+    size = size + g_h.abs()[:, None] * plogp.abs()
+    if d_top is not None:
+        size = size + p * g_top.abs().sum(1)[:, None]
+    nats = 1.0 + torch.nan_to_num(logp.abs(), posinf=0.0).clamp(max=100.0)
+    tol = U * ((3 * SUM + 8 * nats) * size + 4 * direct.abs()) / temperature
+    # the entropy that enters the bracket is float32's
+    tol = tol + p * g_h.abs()[:, None] * scores_tolerance(x, ref, temperature)[1] / temperature
+    return dx, torch.nan_to_num(tol)
+
+
+def close(got, want, tol, dtype=torch.float32):
+    """|got - want| <= tol + one rounding to `dtype`; infinities and NaN in the same places."""
+    got, want = got.detach().double().cpu(), want.double()
+    assert got.shape == want.shape, (got.shape, want.shape)
+    beyond = want.abs() > torch.finfo(dtype).max          # the lowest value over a temperature below one
+    want = torch.where(beyond & torch.isfinite(want), want.sign() * math.inf, want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN in other places"
+    fin = torch.isfinite(want)
+    assert torch.equal(got[~fin & ~torch.isnan(want)], want[~fin & ~torch.isnan(want)]), "infinities differ"
+    bound = torch.as_tensor(tol, dtype=torch.float64).expand(want.shape) * (1 + half_step(dtype))
+    bound = bound + half_step(dtype) * want.abs() + smallest(dtype)
+    off = ((got - want).abs() - bound)[fin]
+    assert off.numel() == 0 or off.max() <= 0, (float(off.max()), float((got - want).abs()[fin].max()))

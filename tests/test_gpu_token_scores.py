@@ -1,0 +1,236 @@
+"""token_scores and its gradient against float64 on the host: sizes around every launch shape,
+masks, ties, rows with nothing left or with NaN, strides, streams, captures, and the run of
+scores into the DDM scan."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import oracle_scan_c
+from lm_reference import close, scores64, scores_grad64, scores_tolerance
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def make(n, v, dtype, seed, special=True):
+    """Logits on the host with every kind of row, and targets on every kind of place."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(n, v, generator=g) * 3).to(dtype)
+    t = torch.randint(0, v, (n,), generator=g)
+    low = torch.finfo(dtype).min
+    if special:
+        for r in range(n):
+            kind = r % 12
+            if kind == 1:
+                x[r] = -math.inf
+            elif kind == 2:
+                x[r] = low
+            elif kind == 3:
+                x[r, torch.rand(v, generator=g) < 0.5] = low
+                x[r, t[r]] = 1.0
+            elif kind == 4:
+                x[r, torch.rand(v, generator=g) < 0.7] = -math.inf
+            elif kind == 5:
+                x[r] = -math.inf
+                x[r, torch.randint(0, v, (1,), generator=g)] = 2.5
+            elif kind == 6:
+                x[r] = 0.75                                     # all equal
+            elif kind == 7:
+                x[r] = torch.randint(-1, 2, (v,), generator=g).to(dtype) * 0.0   # +0 and -0
+            elif kind == 8:
+                x[r] = torch.randint(0, 3, (v,), generator=g).to(dtype)          # many ties
+            elif kind == 9:
+                t[r] = -100
+            elif kind == 10:
+                t[r] = v
+            elif kind == 11:
+                t[r] = v - 1 if r % 2 else 0
+    return x, t
+
+
+def check_scores(x, t, top, temperature, r):
+    ref = scores64(x, t, top, temperature)
+    lp_tol, h_tol = scores_tolerance(x, ref, temperature)
+    n = x.shape[0]
+    assert torch.equal(r.rank.cpu(), ref["rank"])
+    assert torch.equal(r.err.cpu()[:n], ref["err"]) and not r.err.cpu()[n:].any()
+    if top:
+        assert torch.equal(r.top_index.cpu(), ref["top_index"])
+        close(r.top_logprob, ref["top_logprob"], lp_tol(ref["top_logprob"]))
+    else:
+        assert r.top_index is None and r.top_logprob is None
+    close(r.logprob, ref["logprob"], lp_tol(ref["logprob"]))
+    close(r.entropy, ref["entropy"], h_tol)
+    return ref
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,top", [(13, 1, 1), (13, 2, 0), (30, 7, 5), (25, 8, 64), (25, 9, 2), (24, 64, 64),
+                                     (13, 513, 20), (26, 1000, 33), (13, 2049, 7), (13, 4096, 64), (13, 4099, 1),
+                                     (13, 20001, 20), (1, 70001, 64), (3, 131072, 20), (12, 262147, 5)])
+def test_scores(dtype, n, v, top):
+    import ddm_amd
+    x, t = make(n, v, dtype, n * 1000 + v)
+    r = ddm_amd.token_scores(x.cuda(), t.cuda(), top=top)
+    check_scores(x, t, top, 1.0, r)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,top", [(13, 3, 2), (25, 129, 16), (13, 2047, 0), (13, 9001, 64), (2, 50021, 20)])
+@pytest.mark.parametrize("temperature", [0.3, 1.7])
+def test_gradient(dtype, n, v, top, temperature):
+    import ddm_amd
+    x, t = make(n, v, dtype, n + v)
+    g = torch.Generator().manual_seed(v)
+    d = {"d_logprob": torch.randn(n, generator=g), "d_entropy": torch.randn(n, generator=g)}
+    if top:
+        d["d_top"] = torch.randn(n, top, generator=g)
+    xc, tc = x.cuda(), t.int().cuda()
+    r = ddm_amd.token_scores(xc, tc, top=top, temperature=temperature)
+    ref = check_scores(x, t, top, temperature, r)
+    for use in (["d_logprob"], ["d_entropy"], list(d)):
+        given = {k: d[k] for k in use}
+        want, tol = scores_grad64(x, t, ref, temperature, **given)
+        got = ddm_amd.token_scores_grad(xc, tc, r, **{k: a.cuda() for k, a in given.items()})
+        close(got, want, tol, dtype)
+    assert torch.equal(xc.cpu().view(torch.uint8), x.view(torch.uint8))     # read only
+    own = ddm_amd.token_scores_grad(xc, tc, r, **{k: a.cuda() for k, a in d.items()}, out=xc)
+    assert own is xc and torch.equal(own.view(torch.uint8), got.view(torch.uint8))
+
+
+def test_gradient_against_differences():
+    """The reference's own gradient: central differences of its scores in float64."""
+    x, t = make(9, 40, torch.float32, 5, special=False)
+    g = torch.Generator().manual_seed(1)
+    d = {"d_logprob": torch.randn(9, generator=g), "d_entropy": torch.randn(9, generator=g),
+         "d_top": torch.randn(9, 6, generator=g)}
+
+    def total(z):
+        r = scores64(z, t, 6, 0.8)
+        return (d["d_logprob"] * r["logprob"] + d["d_entropy"] * r["entropy"] + (d["d_top"] * r["top_logprob"]).sum(1))
+    z = x.double()
+    want, _ = scores_grad64(z, t, scores64(z, t, 6, 0.8), 0.8, **d)
+    h = 1e-6
+    for c in range(40):
+        e = torch.zeros_like(z)
+        e[:, c] = h
+        diff = (total(z + e) - total(z - e)) / (2 * h)
+        # second order h^2 ~ 1e-12, cancellation 1e-16 * 10 / h = 1e-9
+        assert (diff - want[:, c]).abs().max() < 1e-7
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift,pad", [(0, 8), (1, 5), (3, 0), (7, 9)])
+def test_strides_and_alignment(dtype, shift, pad):
+    import ddm_amd
+    for n, v in ((13, 777), (3, 30011)):
+        x, t = make(n, v, dtype, shift)
+        wide = torch.full((n, shift + v + pad), math.nan, dtype=dtype, device="cuda")
+        view = wide[:, shift:shift + v]
+        view.copy_(x)
+        r = ddm_amd.token_scores(view, t.cuda(), top=9)
+        ref = check_scores(x, t, 9, 1.0, r)
+        out = torch.full((n, v + 3), 7.0, dtype=dtype, device="cuda")
+        d = torch.randn(n, generator=torch.Generator().manual_seed(2))
+        got = ddm_amd.token_scores_grad(view, t.cuda(), r, d_logprob=d.cuda(), out=out[:, 1:v + 1])
+        want, tol = scores_grad64(x, t, ref, 1.0, d_logprob=d)
+        close(got, want, tol, dtype)
+        assert (out[:, 0] == 7).all() and (out[:, v + 1:] == 7).all()
+        assert wide[:, :shift].isnan().all() and wide[:, shift + v:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("where", [0, 511, 12345])
+def test_rows_with_nan_and_infinity(dtype, where):
+    import ddm_amd
+    v = 16385
+    x, t = make(12, v, dtype, 3, special=False)
+    x[1, where] = math.nan
+    x[3, where] = math.inf
+    x[5] = math.nan
+    x[7] = math.inf
+    t[9] = -1
+    x[9, where] = math.nan
+    r = ddm_amd.token_scores(x.cuda(), t.cuda(), top=12)
+    ref = check_scores(x, t, 12, 1.0, r)
+    d = torch.ones(12)
+    want, tol = scores_grad64(x, t, ref, 1.0, d_logprob=d, d_entropy=d)
+    got = ddm_amd.token_scores_grad(x.cuda(), t.cuda(), r, d_logprob=d.cuda(), d_entropy=d.cuda())
+    close(got, want, tol, dtype)
+
+
+def test_no_rows():
+    import ddm_amd
+    x = torch.empty(0, 100, device="cuda")
+    t = torch.empty(0, dtype=torch.int64, device="cuda")
+    r = ddm_amd.token_scores(x, t, top=3)
+    assert r.logprob.shape == (0,) and r.top_index.shape == (0, 3) and r.err.shape == (0,)
+    assert ddm_amd.token_scores_grad(x, t, r, d_logprob=r.logprob).shape == (0, 100)
+
+
+def test_another_stream_and_two_calls_at_once():
+    import ddm_amd
+    x, t = make(40, 33000, torch.bfloat16, 8)
+    xc, tc = x.cuda(), t.cuda()
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    rs = [ddm_amd.token_scores(xc, tc, top=20, stream=s) for s in side]
+    torch.cuda.synchronize()
+    for r in rs:
+        check_scores(x, t, 20, 1.0, r)
+
+
+def test_captured_and_replayed():
+    import ddm_amd
+    xs = [make(5, 40000, torch.bfloat16, k)[0].cuda() for k in range(3)]
+    t = make(5, 40000, torch.bfloat16, 0)[1].cuda()
+    d = torch.randn(5, device="cuda")
+    buf = xs[0].clone()
+
+    def both():
+        r = ddm_amd.token_scores(buf, t, top=8)
+        return r, ddm_amd.token_scores_grad(buf, t, r, d_logprob=d, d_entropy=d)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both()
+    torch.cuda.current_stream().wait_stream(s)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        r1, dx1 = both()
+    with torch.cuda.graph(g2):
+        r2, dx2 = both()
+    for k in range(6):
+        buf.copy_(xs[k % 3])
+        r, dx = both()
+        for g, rg, dg in ((g1, r1, dx1), (g2, r2, dx2)):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(dg.view(torch.int16), dx.view(torch.int16))
+            for a, b in zip(rg[:6], r[:6]):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_scores_into_the_drift_scan(oracle_lib):
+    """A monitored run: the answers get worse half way, the flags go to the scan on the device."""
+    import ddm_amd
+    from ddm_amd import kernels
+    n, v = 3000, 1000
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(n, v, generator=g)
+    t = torch.randint(0, v, (n,), generator=g)
+    right = torch.rand(n, generator=g) < torch.where(torch.arange(n) < n // 2, 0.97, 0.55)
+    x[right, t[right]] += 20.0
+    r = ddm_amd.token_scores(x.to(torch.bfloat16).cuda(), t.cuda())
+    ref = scores64(x.to(torch.bfloat16), t, 0, 1.0)
+    off = torch.tensor([0, n], device="cuda")
+    nb = -(-n // 100)
+    ev = torch.empty(nb, 2, dtype=torch.int32, device="cuda")
+    state = torch.from_numpy(kernels.fresh_states(1).view(np.uint8)).cuda()
+    nev = torch.empty(1, dtype=torch.int64, device="cuda")
+    kernels.scan_streams(r.err, off, kernels.params_struct(), state, torch.zeros(1, dtype=torch.int64, device="cuda"),
+                         nb, ev, nev=nev, mode=1)
+    want, _, _, _ = oracle_scan_c(oracle_lib, ref["err"].numpy(), np.array([0, n]), mode=1)
+    assert np.array_equal(ev.cpu().numpy(), want) and (want[:, 1] >= 0).any()
