@@ -3,6 +3,8 @@
 #pragma once
 #include <float.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace ddm {
@@ -202,6 +204,70 @@ __device__ __forceinline__ float below(float x) {
 
 __device__ __forceinline__ int64_t target_at(const void* t, int wide, int64_t i) {
     return wide ? ((const int64_t*)t)[i] : (int64_t)((const int32_t*)t)[i];
+}
+
+constexpr int kMaxTop = 64;              // alternatives of a row: one a lane
+constexpr int kMaxParts = 64;            // parts of a row, as well
+constexpr int64_t kMaxColumns = 1 << 19;
+
+// Lanes a workgroup, vectors a lane, workgroups a row.
+struct Shape {
+    int nt, nv, parts;
+};
+template <typename F>
+int with_type(int32_t dtype, F f) {
+    switch (dtype) {
+        case DDM_F32: return f(f32_t());
+        case DDM_BF16: return f(bf16_t());
+        case DDM_F16: return f(f16_t());
+    }
+    return DDM_E_ARG;
+}
+#define DDM_SHAPE(NT_, NV_) \
+    if (s.nt == NT_ && s.nv == NV_) return f(std::integral_constant<int, NT_>(), std::integral_constant<int, NV_>())
+template <typename F>
+void with_part_shape(const Shape& s, F f) {
+    DDM_SHAPE(64, 1);
+    DDM_SHAPE(64, 2);
+    DDM_SHAPE(64, 4);
+    DDM_SHAPE(64, 8);
+    DDM_SHAPE(256, 1);
+    DDM_SHAPE(256, 2);
+    DDM_SHAPE(256, 4);
+    DDM_SHAPE(256, 8);
+}
+template <typename F>
+void with_row_shape(const Shape& s, F f) {
+    DDM_SHAPE(64, 1);
+    DDM_SHAPE(64, 2);
+    DDM_SHAPE(64, 4);
+    DDM_SHAPE(64, 8);
+    DDM_SHAPE(256, 4);
+    DDM_SHAPE(256, 8);
+    DDM_SHAPE(1024, 4);
+    DDM_SHAPE(1024, 8);
+    DDM_SHAPE(1024, 16);
+}
+#undef DDM_SHAPE
+
+// The checks the entry points share; 0 or DDM_E_ARG with the reason.
+inline int check_rows(const char* who, int32_t dtype, int64_t n, int64_t v, int64_t ld, int32_t target_bytes,
+                      float temperature, int32_t top) {
+    if (dtype != DDM_F32 && dtype != DDM_BF16 && dtype != DDM_F16) {
+        set_error("%s: unknown type %d", who, (int)dtype);
+    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts) {
+        set_error("%s: invalid argument (rows %lld, columns %lld of 1..%lld, row stride %lld)", who, (long long)n,
+                  (long long)v, (long long)kMaxColumns, (long long)ld);
+    } else if (target_bytes != 4 && target_bytes != 8) {
+        set_error("%s: targets of %d bytes (4 or 8)", who, (int)target_bytes);
+    } else if (!(temperature > 0.0f) || !(temperature < INFINITY)) {
+        set_error("%s: temperature must be positive and finite", who);
+    } else if (top < 0 || top > kMaxTop) {
+        set_error("%s: %d alternatives (0..%d)", who, (int)top, kMaxTop);
+    } else {
+        return 0;
+    }
+    return DDM_E_ARG;
 }
 
 }  // namespace logits

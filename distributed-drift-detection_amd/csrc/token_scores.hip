@@ -11,16 +11,12 @@
 // few rows are cut finer, until there are enough workgroups for the chip.  Parts meet in a
 // second small launch.  No atomic decides an order: every sum is a fixed tree, and the
 // alternatives are ordered by (value, index).
-#include <type_traits>
-
 #include "logits.h"
 
 namespace ddm {
 namespace logits {
 
-constexpr int kMaxTop = 64;
 constexpr int kListCap = 512;        // candidates a selection keeps in LDS
-constexpr int kMaxParts = 64;        // parts of a row
 
 struct ScoreArgs {
     const char* x;
@@ -415,9 +411,6 @@ __global__ __launch_bounds__(NT) void k_score_grad(GradArgs a) {
 // One wave a row while the row fits its registers (512 vectors of 16 bytes); longer rows in
 // parts of 256 lanes, 8 vectors each, or fewer while there are not workgroups enough to fill
 // 256 CUs several times over.
-struct Shape {
-    int nt, nv, parts;
-};
 inline Shape shape_of(int64_t n, int64_t v, int vec) {
     const int64_t nvec = ceil_div(v + vec - 1, vec);     // whatever the rows' alignment
     Shape s;
@@ -431,52 +424,6 @@ inline Shape shape_of(int64_t n, int64_t v, int vec) {
     }
     s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv);
     return s;
-}
-
-constexpr int64_t kMaxColumns = 1 << 19;
-
-template <typename F>
-int with_type(int32_t dtype, F f) {
-    switch (dtype) {
-        case DDM_F32: return f(f32_t());
-        case DDM_BF16: return f(bf16_t());
-        case DDM_F16: return f(f16_t());
-    }
-    return DDM_E_ARG;
-}
-template <typename F>
-void with_shape(const Shape& s, F f) {
-#define DDM_SHAPE(NT_, NV_) \
-    if (s.nt == NT_ && s.nv == NV_) return f(std::integral_constant<int, NT_>(), std::integral_constant<int, NV_>())
-    DDM_SHAPE(64, 1);
-    DDM_SHAPE(64, 2);
-    DDM_SHAPE(64, 4);
-    DDM_SHAPE(64, 8);
-    DDM_SHAPE(256, 1);
-    DDM_SHAPE(256, 2);
-    DDM_SHAPE(256, 4);
-    DDM_SHAPE(256, 8);
-#undef DDM_SHAPE
-}
-
-// The checks both entry points share; 0 or DDM_E_ARG with the reason.
-inline int check_rows(const char* who, int32_t dtype, int64_t n, int64_t v, int64_t ld, int32_t target_bytes,
-                      float temperature, int32_t top) {
-    if (dtype != DDM_F32 && dtype != DDM_BF16 && dtype != DDM_F16) {
-        set_error("%s: unknown type %d", who, (int)dtype);
-    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts) {
-        set_error("%s: invalid argument (rows %lld, columns %lld of 1..%lld, row stride %lld)", who, (long long)n,
-                  (long long)v, (long long)kMaxColumns, (long long)ld);
-    } else if (target_bytes != 4 && target_bytes != 8) {
-        set_error("%s: targets of %d bytes (4 or 8)", who, (int)target_bytes);
-    } else if (!(temperature > 0.0f) || !(temperature < INFINITY)) {
-        set_error("%s: temperature must be positive and finite", who);
-    } else if (top < 0 || top > kMaxTop) {
-        set_error("%s: %d alternatives (0..%d)", who, (int)top, kMaxTop);
-    } else {
-        return 0;
-    }
-    return DDM_E_ARG;
 }
 
 }  // namespace logits
@@ -511,7 +458,7 @@ extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, in
             ScoreArgs a{(const char*)logits, n, v, ld * T::kSize, target, target_bytes == 8, temperature, top, s.parts,
                         logprob, entropy, stats, top_logprob, rank, top_index, err, (float4*)scratch,
                         (uint64_t*)((char*)scratch + n * s.parts * 16)};
-            with_shape(s, [&](auto nt, auto nv) {
+            with_part_shape(s, [&](auto nt, auto nv) {
                 if (top)
                     k_score_parts<T, nt(), nv(), true><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
                 else
@@ -547,7 +494,7 @@ extern "C" int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t 
             using T = decltype(type);
             GradArgs a{(const char*)logits, n, v, ld * T::kSize, out_ld * T::kSize, target, target_bytes == 8,
                        temperature, top, s.parts, stats, entropy, top_index, d_logprob, d_entropy, d_top, (char*)out};
-            with_shape(s, [&](auto nt, auto nv) {
+            with_part_shape(s, [&](auto nt, auto nv) {
                 k_score_grad<T, nt(), nv()><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
             });
             return launch_status("ddm_token_scores_grad");

@@ -188,3 +188,45 @@ def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d
                                         _ptr(d_top), out.data_ptr(), out_ld, s, *_evs(timer)),
               "ddm_token_scores_grad")
     return out
+
+
+TAILS = {"renorm": 0, "rest": 1}
+
+
+def topk_distill(logits, index, logprob, tail="rest", temperature=1.0, weight=None, grad=False, out=None, stream=None,
+                 timer=None):
+    """Loss [n] (float32) of a student's logits [n, v] against a teacher's alternatives: index
+    [n, k] (int32 or int64) with their log probabilities [n, k] (float32), k at most 64, as
+    token_scores gives them.  Indexes outside [0, v) are none, and repeats of an earlier one too.
+
+    tail "rest": what the alternatives leave of the teacher's probability is one more outcome,
+    "none of these" (temperature 1); "renorm": the alternatives alone, softened by the
+    temperature.  grad (or out, a tensor like token_scores_grad's): also the gradient of
+    weight . loss (float32 [n], None: ones) by the logits, from the same reading.  Returns (loss,
+    gradient or None)."""
+    n, v, ld = _logits(logits)
+    if tail not in TAILS:
+        raise ValueError(f"tail must be one of {', '.join(TAILS)}, got {tail!r}")
+    temperature = _temperature(temperature)
+    if tail == "rest" and temperature != 1.0:
+        raise ValueError("tail 'rest' is known at temperature 1 only")
+    if not isinstance(index, torch.Tensor) or index.dim() != 2 or index.shape[1] > MAX_TOP:
+        raise ValueError(f"index must be a tensor [n, k] with k at most {MAX_TOP}")
+    k = index.shape[1]
+    shaped("index", index, (n, k), torch.int32, torch.int64)
+    shaped("logprob", logprob, (n, k), torch.float32)
+    if weight is not None:
+        shaped("weight", weight, (n,), torch.float32)
+    _check_out(out, logits)
+    code = DTYPES[logits.dtype]
+    with launch_on(logits, stream, (logits, index, logprob, weight, out)) as s:
+        index, logprob, weight = dense(index), dense(logprob), dense(weight)
+        loss = torch.empty(n, dtype=torch.float32, device=logits.device)
+        out = _new_like(out, logits) if grad or out is not None else None
+        need = int(lib.ddm_topk_distill_scratch_bytes(n, v, code, k, out is not None))
+        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        out_ld = v if out is None or n <= 1 else out.stride(0)
+        check(lib.ddm_topk_distill(logits.data_ptr(), code, n, v, ld, index.data_ptr(), index.element_size(),
+                                   logprob.data_ptr(), k, TAILS[tail], temperature, _ptr(weight), loss.data_ptr(),
+                                   _ptr(out), out_ld, _ptr(scratch), s, *_evs(timer)), "ddm_topk_distill")
+    return loss, out

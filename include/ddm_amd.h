@@ -772,6 +772,27 @@ int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t n, int64_t 
                           const float* d_entropy, const float* d_top, void* out, int64_t out_ld,
                           ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
 
+/* The loss of a student's logits (n rows of v, as above) against a teacher's alternatives:
+ * index[n * k] (index_bytes 4 or 8) and their log probabilities logprob[n * k] over the whole
+ * vocabulary, k at most 64 (ddm_token_scores' top_index and top_logprob).  An index outside
+ * [0, v) is none, and so is the repeat of an earlier one.  tail:
+ *   DDM_TAIL_RENORM  q = softmax(logprob / T) over what is given, loss = sum q (log q - log p)
+ *   DDM_TAIL_REST    T = 1: q = exp(logprob), and what is missing to 1 (if 2^-20 or more) stands
+ *                    for all other columns together, as one more term
+ * loss[n], float32, +inf where the teacher expects what the student excludes, 0 where nothing
+ * is given (renorm), NaN for a row with NaN or +inf.  grad (NULL: the loss alone): the gradient
+ * of sum weight loss (weight[n], NULL: 1) in the logits' type, row stride grad_ld; the logits'
+ * own buffer with their stride, or one apart from it.  Rows of weight 0, and rows of -inf alone,
+ * have gradient 0.  scratch: ddm_topk_distill_scratch_bytes(...) bytes, 16-byte aligned (NULL
+ * if 0). */
+#define DDM_TAIL_RENORM 0
+#define DDM_TAIL_REST   1
+int64_t ddm_topk_distill_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t k, int32_t grad);
+int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld, const void* index,
+                     int32_t index_bytes, const float* logprob, int32_t k, int32_t tail, float temperature,
+                     const float* weight, float* loss, void* grad, int64_t grad_ld, void* scratch,
+                     ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
+
 /* ---- synthetic inputs (benchmark configs) ------------------------- */
 
 /* Labels of a class-block stream partitioned as DDM_Process.py:225 (row % n_parts):

@@ -119,3 +119,64 @@ def close(got, want, tol, dtype=torch.float32):
     bound = bound + half_step(dtype) * want.abs() + smallest(dtype)
     off = ((got - want).abs() - bound)[fin]
     assert off.numel() == 0 or off.max() <= 0, (float(off.max()), float((got - want).abs()[fin].max()))
+
+
+def first_of_each(index, v):
+    """Which entries count: inside the row, and no repeat of an earlier one."""
+    inside = (index >= 0) & (index < v)
+    same = (index[:, :, None] == index[:, None, :]).tril(-1).any(2)
+    return inside & ~same
+
+
+def distill64(x, index, logprob, tail, temperature, weight=None):
+    """(loss, its bound, gradient, its bound) in float64."""
+    n, v = x.shape
+    logp, dead, bad = softmax64(x, temperature)
+    keep = first_of_each(index, v)
+    head = torch.zeros(n, v, dtype=torch.bool)
+    logq = torch.full((n, v), -math.inf, dtype=torch.float64)
+    for r in range(n):
+        cols = index[r][keep[r]].long()
+        head[r, cols] = True
+        logq[r, cols] = logprob[r][keep[r]].double()
+    given = logq.clone()
+    if tail == "renorm":
+        logq = logq / temperature
+        top = logq.amax(1, keepdim=True)
+        some = top > -math.inf
+        logq = torch.where(some, logq - top, -math.inf)
+        logq = logq - torch.where(some, logq.exp().sum(1, keepdim=True).log(), 0.0)
+        rest = torch.zeros(n, 1, dtype=torch.float64)
+    else:
+        rest = 1.0 - logq.exp().sum(1, keepdim=True)
+        rest = torch.where((rest < 2.0 ** -20) | (head.sum(1, keepdim=True) == v), 0.0, rest)
+    q = logq.exp()
+    log_rest = torch.logsumexp(torch.where(head, -math.inf, logp), 1, keepdim=True)
+    gap = torch.where(q > 0, logq - logp, 0.0)
+    last = torch.where(rest > 0, rest.log() - log_rest, 0.0)
+    loss = (torch.where(q > 0, q * gap, 0.0).sum(1, keepdim=True) + torch.where(rest > 0, rest * last, 0.0))[:, 0]
+    loss = torch.where(bad, math.nan, loss)
+    calm = lambda t: torch.nan_to_num(t, nan=0.0, posinf=0.0, neginf=0.0).abs()  # noqa: E731
+    log_v = math.log(v) + 1.0
+    # log p: a sum and two nats' roundings; q: its exponential and normalisation; the remainder:
+    # a difference with 12 half steps of 1
+    tol = (q * (SUM + 20 + 3 * log_v + 4 * calm(logp) + 16 * calm(gap) + 4 * calm(given / temperature))).sum(1)
+    tol = tol + 12 * (calm(last)[:, 0] + 1) + (rest * (2 * SUM + 6 * log_v + 4 * calm(log_rest)))[:, 0]
+    p = logp.exp()
+    share = torch.where(head | torch.isneginf(log_rest), 0.0, (logp - log_rest).exp())
+    w = torch.ones(n, 1, dtype=torch.float64) if weight is None else weight.double()[:, None]
+    whole = q.sum(1, keepdim=True) + rest
+    dx = torch.where(head, p * whole - q, p * whole - rest * share)
+    nats = 1.0 + calm(logp).clamp(max=100.0)
+    p_rest = log_rest.exp()
+    head_tol = p * (2 * SUM + 8 * nats + 24) + q * (24 + 8 * calm(given / temperature) + 8 * calm(logq))
+    if tail == "rest":
+        bulk_tol = share * ((SUM + 8 * nats + 8 * calm(log_rest)) * (p_rest * whole - rest).abs()
+                            + p_rest * (2 * SUM + 8 * calm(log_rest) + 24) + 16)
+    else:
+        bulk_tol = p * (2 * SUM + 8 * nats + 24)
+    none = dead[:, None] | (w == 0)
+    dx = torch.where(none, 0.0, torch.where(bad[:, None], math.nan, dx)) * w / temperature
+    dx = torch.where(none, 0.0, dx)
+    dx_tol = U * torch.nan_to_num(torch.where(head, head_tol, bulk_tol)) * w.abs() / temperature
+    return loss, U * torch.nan_to_num(tol), dx, dx_tol

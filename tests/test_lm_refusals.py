@@ -77,3 +77,39 @@ def test_entry_points_check_before_they_launch():
                                            None, None, None) == _capi.DDM_E_ARG and "stride" in last_error()
     assert _capi.lib.ddm_token_scores_scratch_bytes(4, 100, 0, 3) == 0
     assert _capi.lib.ddm_token_scores_scratch_bytes(4, 100000, 0, 3) > 0
+
+
+I, LP = torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, 3)
+
+
+@pytest.mark.parametrize("args,kw,error", [
+    ((X, I, LP), {}, "on the GPU"),
+    ((X, I, LP), {"tail": "head"}, "tail"),
+    ((X, I, LP), {"temperature": 2.0}, "temperature 1"),
+    ((X, I, LP), {"tail": "renorm", "temperature": -1.0}, "temperature"),
+    ((X, I[0], LP), {}, "index"),
+    ((X, I[:3], LP), {}, "index"),
+    ((X, I.float(), LP), {}, "index"),
+    ((X, torch.zeros(4, 65, dtype=torch.int32), torch.zeros(4, 65)), {}, "index"),
+    ((X, I, LP[:, :2]), {}, "logprob"),
+    ((X, I, LP.double()), {}, "logprob"),
+    ((X, I, LP), {"weight": torch.zeros(3)}, "weight"),
+    ((X, I, LP), {"out": torch.zeros(4, 11)}, "out"),
+])
+def test_topk_distill(args, kw, error):
+    with pytest.raises((ValueError, TypeError), match=error):
+        tokens.topk_distill(*args, **kw)
+
+
+def test_distill_entry_point_checks_before_it_launches():
+    one = ctypes.c_void_p(256)
+
+    def distill(k=3, tail=0, temp=1.0, index=one, grad=None, grad_ld=10, v=10, ld=10):
+        return _capi.lib.ddm_topk_distill(one, 0, 4, v, ld, index, 4, one, k, tail, temp, None, one, grad, grad_ld,
+                                          None, None, None, None)
+    for kw, text in (({"k": 65}, "alternatives"), ({"tail": 2}, "tail"), ({"tail": 1, "temp": 2.0}, "temperature 1"),
+                     ({"index": None}, "null"), ({"grad": one, "grad_ld": 9}, "gradient stride"),
+                     ({"v": 100000, "ld": 100000}, "null")):
+        assert distill(**kw) == _capi.DDM_E_ARG and text in last_error(), (kw, last_error())
+    assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100, 0, 3, 1) == 0
+    assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100000, 0, 3, 1) > 0
