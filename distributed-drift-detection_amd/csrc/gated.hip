@@ -1,0 +1,248 @@
+// The recurrence forwards, and its single step (the method: gated.h).
+#include "gated.h"
+
+namespace ddm {
+namespace gated {
+
+// ---- forward ----------------------------------------------------------------------------------------
+template <typename X, typename L, int VEC, bool OWN, int R>
+__global__ __launch_bounds__(NT) void k_gated_scan(Args a) {
+    extern __shared__ int32_t marks[];
+    __shared__ ScanLds<VEC> lds;
+    const Place at = take(a);
+    const int cl = 1 << a.cl_bits, tg = threadIdx.x >> a.cl_bits, tr = (NT >> a.cl_bits) * R;
+    const int c = (at.block * cl + (int)(threadIdx.x & (cl - 1))) * VEC;
+    const int64_t row0 = at.tile * tr, r0 = row0 + tg * R;
+    const bool active = c < a.d;
+    Raw<X, VEC> x[R];
+    Gates<L, VEC, OWN> l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (active && r0 + r < a.rows) {
+            x[r] = load<X, VEC>(a.x, a.ld_x, r0 + r, c);
+            l[r].load_row(a, r0 + r, c);
+        }
+    }
+    int32_t *begins = marks, *ends = marks + tr;
+    int64_t first = 0, end = a.rows;
+    if (a.off) {
+        mark_rows(a, row0, tr, begins, ends);
+        first = a.off[0];
+        end = a.off[a.n];
+        end = end < a.rows ? end : a.rows;
+    }
+    float b[R][VEC];
+    uint32_t cut = 0;                                // rows whose state before is no factor
+    Step own[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t row = r0 + r;
+        const bool inside = active && row >= first && row < end;
+        const int s = !inside ? -1 : a.off ? begins[tg * R + r] : row == 0 ? 0 : -1;
+        if (!inside || s >= 0) cut |= 1u << r;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float g = 0.0f, y = 0.0f;
+            if (inside) {
+                const float lv = l[r][v];
+                g = gate(lv);
+                y = input_factor(lv, a.scale) * (float)x[r].e[v];
+                if (s >= 0 && a.state_in) y = fmaf(g, a.state_in[(int64_t)s * a.d + c + v], y);
+            }
+            b[r][v] = y;
+            own[v] = after(own[v], Step{cut >> r & 1 ? kCut : g, y});
+        }
+    }
+    float h[VEC];
+    chain<VEC>(a, at, own, lds, h);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t row = r0 + r;
+        const bool inside = active && row >= first && row < end;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = cut >> r & 1 ? b[r][v] : fmaf(gate(l[r][v]), h[v], b[r][v]);
+        if (inside || (a.fill && active && row < a.rows)) store<X, VEC>(a.out, a.ld_h, row, c, h);
+        const int s = !inside ? -1 : a.off ? ends[tg * R + r] : row == a.rows - 1 ? 0 : -1;
+        if (s >= 0) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) a.state_out[(int64_t)s * a.d + c + v] = h[v];
+        }
+    }
+}
+
+// Before a scan: what the chain waits for is unset, and every sequence's state goes through
+// (those with rows write theirs afterwards).
+__global__ __launch_bounds__(256) void k_gated_begin(uint32_t* ticket, uint64_t* words, int64_t nwords,
+                                                     const float* from, float* to, int64_t nstate) {
+    const int64_t step = (int64_t)gridDim.x * 256;
+    const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i0 == 0 && ticket) *ticket = 0;
+    for (int64_t i = i0; i < nwords; i += step) words[i] = kUnset;
+    for (int64_t i = i0; i < nstate; i += step) to[i] = from ? from[i] : 0.0f;
+}
+
+// One row a sequence: elementwise, the state's row beside it.
+template <typename X, typename L, int VEC, bool OWN>
+__global__ __launch_bounds__(256) void k_gated_step(Args a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int per = a.d / VEC;
+    const int64_t row = i / per;
+    const int c = (int)(i % per) * VEC;
+    if (row >= a.rows) return;
+    const Raw<X, VEC> x = load<X, VEC>(a.x, a.ld_x, row, c);
+    Gates<L, VEC, OWN> l;
+    l.load_row(a, row, c);
+    float h[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        const float before = a.state_in ? a.state_in[row * a.d + c + v] : 0.0f;
+        h[v] = fmaf(gate(l[v]), before, input_factor(l[v], a.scale) * (float)x.e[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) a.state_out[row * a.d + c + v] = h[v];
+    store<X, VEC>(a.out, a.ld_h, row, c, h);
+}
+
+// The chain's buffers, the copy of the states, and where both are needed their launch.
+int begin(Args& a, const Shape& s, void* scratch, const float* from, float* to, int64_t nstate, hipStream_t st) {
+    char* w = (char*)scratch;
+    const int64_t words = s.words();
+    if (words) {
+        a.ticket = (uint32_t*)w;
+        a.agg = (uint64_t*)(w + 16);
+        a.inc = a.agg + s.ntiles * s.dp;
+        w += 16 + 8 * words;
+    }
+    if (s.dl_parts) a.dl_part = (float*)w;
+    a.cl_bits = s.cl_bits;
+    a.ncb = s.ncb;
+    a.group = s.group;
+    a.ntiles = s.ntiles;
+    a.dp = s.dp;
+    a.dl_width = s.dl_width;
+    const int64_t most = words > nstate ? words : nstate;
+    if (!words && !a.off && s.ntiles) return 0;        // one tile, one sequence that has rows
+    const int64_t grid = ceil_div(most, 256 * 4) < 2048 ? ceil_div(most, 256 * 4) : 2048;
+    k_gated_begin<<<dim3((unsigned)(grid > 0 ? grid : 1)), 256, 0, st>>>(a.ticket, a.agg, words, from, to, nstate);
+    return launch_status("ddm_gated_scan");
+}
+
+}  // namespace gated
+}  // namespace ddm
+
+using namespace ddm;
+using namespace ddm::gated;
+
+extern "C" int64_t ddm_gated_scan_scratch_bytes(int64_t rows, int64_t d, int64_t gates, int32_t dtype, int32_t grad) {
+    if (rows <= 0 || d < 1 || d > 1 << 20 || gates < 1 || d % gates || dtype < 0 || dtype > DDM_F16) return 0;
+    // whichever way the operands are aligned
+    int64_t most = 0;
+    for (int vec : {1, wide_vec(dtype)})
+        if (d % vec == 0 && (gates == d || d / gates % vec == 0)) {
+            const int64_t b = scratch_bytes(shape_of(rows, (int)d, (int)(d / gates), vec, grad != 0), rows, (int)d);
+            most = b > most ? b : most;
+        }
+    return most;
+}
+
+extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const void* log_a, int32_t gate_dtype,
+                              int64_t ld_a, int64_t rows, int64_t d, int64_t gates, const int64_t* offsets, int64_t n,
+                              int32_t scale, const float* state_in, float* state_out, void* out, int64_t ld_out,
+                              int32_t fill, void* scratch, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end) {
+    if (int rc = check("ddm_gated_scan", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, n, scale)) return rc;
+    if ((rows && (!x || !log_a || !out || ld_out < d)) || (n && !state_out) || (!offsets && n != 1) ||
+        (state_in && state_in == state_out)) {
+        set_error("ddm_gated_scan: invalid argument (null pointer, output stride, one sequence without offsets, or the "
+                  "states in one buffer)");
+        return DDM_E_ARG;
+    }
+    const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype);
+    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
+    const Shape s = shape_of(rows, (int)d, share, vec, false);
+    if (int rc = check_grid("ddm_gated_scan", s)) return rc;
+    if (scratch_bytes(s, rows, (int)d) && !scratch) {
+        set_error("ddm_gated_scan: invalid argument (no scratch)");
+        return DDM_E_ARG;
+    }
+    const hipStream_t st = as_hip(stream);
+    return timed(ev_begin, ev_end, st, [&]() -> int {
+        Args a{};
+        a.x = (const char*)x;
+        a.l = (const char*)log_a;
+        a.out = (char*)out;
+        a.ld_x = ld_x * es;
+        a.ld_l = ld_a * gs;
+        a.ld_h = ld_out * es;
+        a.rows = rows;
+        a.d = (int)d;
+        a.share = share;
+        a.scale = scale;
+        a.fill = fill;
+        a.off = offsets;
+        a.n = n;
+        a.state_in = state_in;
+        a.state_out = state_out;
+        if (int rc = begin(a, s, scratch, state_in, state_out, n * d, st)) return rc;
+        if (rows == 0) return 0;
+        const size_t lds = offsets ? (size_t)(NT >> s.cl_bits) * s.r * 8 : 0;
+        return with_types(dtype, gate_dtype, [&](auto xt, auto lt) {
+            using X = decltype(xt);
+            using L = decltype(lt);
+            with_vec(vec, share == 1, [&](auto v, auto own) {
+                constexpr int V = v() ? 1 : 8 / (int)sizeof(typename X::E);
+                const dim3 grid((unsigned)(s.ntiles * s.ncb));
+                if (s.r == 16)
+                    k_gated_scan<X, L, V, own(), 16><<<grid, NT, lds, st>>>(a);
+                else
+                    k_gated_scan<X, L, V, own(), 4><<<grid, NT, lds, st>>>(a);
+            });
+            return launch_status("ddm_gated_scan");
+        });
+    });
+}
+
+extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const void* log_a, int32_t gate_dtype,
+                              int64_t ld_a, int64_t rows, int64_t d, int64_t gates, int32_t scale, const float* state_in,
+                              float* state_out, void* out, int64_t ld_out, ddm_stream_t stream, ddm_event_t ev_begin,
+                              ddm_event_t ev_end) {
+    if (int rc = check("ddm_gated_step", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, rows, scale)) return rc;
+    if (rows == 0) return 0;
+    if (!x || !log_a || !state_out || !out || ld_out < d) {
+        set_error("ddm_gated_step: invalid argument (null pointer or output stride)");
+        return DDM_E_ARG;
+    }
+    const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype);
+    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
+    const int64_t blocks = ceil_div(rows * (d / vec), 256);
+    if (blocks > INT32_MAX) {
+        set_error("ddm_gated_step: %lld rows of %lld channels", (long long)rows, (long long)d);
+        return DDM_E_ARG;
+    }
+    const hipStream_t st = as_hip(stream);
+    return timed(ev_begin, ev_end, st, [&] {
+        Args a{};
+        a.x = (const char*)x;
+        a.l = (const char*)log_a;
+        a.out = (char*)out;
+        a.ld_x = ld_x * es;
+        a.ld_l = ld_a * gs;
+        a.ld_h = ld_out * es;
+        a.rows = rows;
+        a.d = (int)d;
+        a.share = share;
+        a.scale = scale;
+        a.state_in = state_in;
+        a.state_out = state_out;
+        return with_types(dtype, gate_dtype, [&](auto xt, auto lt) {
+            using X = decltype(xt);
+            using L = decltype(lt);
+            with_vec(vec, share == 1, [&](auto v, auto own) {
+                constexpr int V = v() ? 1 : 8 / (int)sizeof(typename X::E);
+                k_gated_step<X, L, V, own()><<<dim3((unsigned)blocks), 256, 0, st>>>(a);
+            });
+            return launch_status("ddm_gated_step");
+        });
+    });
+}

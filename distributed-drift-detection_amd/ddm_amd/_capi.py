@@ -159,6 +159,14 @@ SIGNATURES = {
     "ddm_topk_distill_scratch_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32]),
     "ddm_topk_distill": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _f32, _vp, _vp, _vp,
                                         _i64, _vp, _vp, _vp, _vp]),
+    "ddm_gated_scan_scratch_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
+    "ddm_gated_scan": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp,
+                                      _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "ddm_gated_scan_grad": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                                           _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp,
+                                           _vp]),
+    "ddm_gated_step": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64,
+                                      _vp, _vp, _vp]),
     "ddm_synth_block_labels": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i32, _vp]),
     "ddm_synth_jitter_labels": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i32, ctypes.c_double, _u64,
                                                _vp]),

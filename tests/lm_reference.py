@@ -180,3 +180,66 @@ def distill64(x, index, logprob, tail, temperature, weight=None):
     dx = torch.where(none, 0.0, dx)
     dx_tol = U * torch.nan_to_num(torch.where(head, head_tol, bulk_tol)) * w.abs() / temperature
     return loss, U * torch.nan_to_num(tol), dx, dx_tol
+
+
+def gated64(x, log_a, offsets, state, scale, h_given=None, d_h=None, d_state=None):
+    """The recurrence a row at a time in float64, with bounds of what float32 may differ by.
+
+    A step costs an exponential, the factor, a product and a sum, and their regrouping as much
+    again: under STEP = 10 half steps of the majorant H_t = a H_{t-1} + |b_t|, which also bounds
+    what any grouping of the steps adds up on the way.  Returns dicts of (value, bound)."""
+    import numpy as np
+    step = 10 * U
+    rows, d = x.shape
+    g = log_a.shape[1]
+    xd, lam = x.double().numpy(), np.repeat(log_a.double().numpy(), d // g, 1)
+    a = np.exp(lam)
+    with np.errstate(all="ignore"):
+        if scale == "none":
+            f, df = np.ones_like(a), np.zeros_like(a)
+        elif scale == "ewma":
+            f, df = -np.expm1(lam), -a
+        else:
+            f = np.sqrt(np.maximum(-np.expm1(2 * lam), 0))
+            df = np.where(f > 0, -a * a / np.where(f > 0, f, 1), 0.0)
+    off = [0, rows] if offsets is None else offsets.tolist()
+    n = len(off) - 1
+    h0 = np.zeros((n, d)) if state is None else state.double().numpy()
+    h, ht = np.zeros((rows, d)), np.zeros((rows, d))
+    s, st = h0.copy(), np.zeros((n, d))
+    b = f * xd
+    ab = np.abs(b)
+    for q in range(n):
+        c, m, t = h0[q], np.abs(h0[q]), np.zeros(d)
+        for r in range(off[q], off[q + 1]):
+            c = a[r] * c + b[r]
+            m = a[r] * m + ab[r]
+            t = a[r] * t + step * m
+            h[r], ht[r] = c, t
+        s[q], st[q] = c, t
+    pair = lambda v, t: (torch.from_numpy(v), torch.from_numpy(t))  # noqa: E731
+    out = {"h": pair(h, ht), "state": pair(s, st)}
+    if d_h is None:
+        return out
+    hg, dh = h_given.double().numpy(), d_h.double().numpy()
+    ds = np.zeros((n, d)) if d_state is None else d_state.double().numpy()
+    dx, dxt, dl, dlt = (np.zeros((rows, d)) for _ in range(4))
+    d0, d0t = ds.copy(), np.zeros((n, d))
+    for q in range(n):
+        c, m, t = ds[q], np.abs(ds[q]), np.zeros(d)
+        for r in range(off[q + 1] - 1, off[q] - 1, -1):
+            c, m = c + dh[r], m + np.abs(dh[r])
+            t = t + step * m
+            before = hg[r - 1] if r > off[q] else h0[q]
+            dx[r], dxt[r] = c * f[r], (t + step * m) * f[r]
+            parts = np.abs(a[r] * before) + np.abs(df[r] * xd[r])
+            dl[r], dlt[r] = c * (a[r] * before + df[r] * xd[r]), (t + 2 * step * m) * parts
+            c, m, t = a[r] * c, a[r] * m, a[r] * t + step * a[r] * m
+        d0[q], d0t[q] = c, t
+    share = d // g
+    if share > 1:                               # one gate's sum, in any order
+        size = np.abs(dl).reshape(rows, g, share).sum(2)
+        dl = dl.reshape(rows, g, share).sum(2)
+        dlt = dlt.reshape(rows, g, share).sum(2) + U * share * size
+    out.update(d_x=pair(dx, dxt), d_log_a=pair(dl, dlt), d_state=pair(d0, d0t))
+    return out

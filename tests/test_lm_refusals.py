@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from ddm_amd import _capi, tokens
+from ddm_amd import _capi, gated, tokens
 
 X = torch.zeros(4, 10)
 T = torch.zeros(4, dtype=torch.int64)
@@ -113,3 +113,97 @@ def test_distill_entry_point_checks_before_it_launches():
         assert distill(**kw) == _capi.DDM_E_ARG and text in last_error(), (kw, last_error())
     assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100, 0, 3, 1) == 0
     assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100000, 0, 3, 1) > 0
+
+
+G = torch.zeros(4, 5)
+OFF = torch.zeros(3, dtype=torch.int64)
+S = torch.zeros(2, 10)
+
+
+@pytest.mark.parametrize("args,kw,error", [
+    ((X, G), {}, "on the GPU"),
+    ((X, G[:1].expand(4, 5)), {}, "on the GPU"),
+    ((X, torch.zeros(4, 3)), {}, "dividing"),
+    ((X, torch.zeros(3, 5)), {}, "log_a"),
+    ((X, torch.zeros(4, 0)), {}, "log_a"),
+    ((X, G.to(torch.bfloat16)), {}, "log_a"),
+    ((X.to(torch.bfloat16), G.to(torch.float16)), {}, "log_a"),
+    ((X.double(), G), {}, "type"),
+    ((X.t(), torch.zeros(10, 4)), {}, "contiguous"),
+    ((torch.zeros(4, 0), G), {}, "channels"),
+    ((X, G), {"scale": "max"}, "scale"),
+    ((X, G), {"offsets": OFF.int()}, "offsets"),
+    ((X, G), {"offsets": [0, 4]}, "offsets"),
+    ((X, G), {"offsets": OFF[:0]}, "offsets"),
+    ((X, G), {"offsets": OFF, "state": S[:1]}, "state"),
+    ((X, G), {"state": S}, "state"),
+    ((X, G), {"offsets": OFF, "state": S.double()}, "state"),
+    ((X, G), {"out": torch.zeros(4, 9)}, "out"),
+    ((X, torch.zeros(4, 10)), {"out": "log_a"}, "overlaps"),
+])
+def test_gated_scan(args, kw, error):
+    if kw.get("out") == "log_a":
+        kw = {"out": args[1]}
+    with pytest.raises((ValueError, TypeError), match=error):
+        gated.gated_scan(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw,error", [
+    ((X, G, X, X), {}, "on the GPU"),
+    ((X, G, X[:3], X), {}, "h must"),
+    ((X, G, X, X.double()), {}, "d_h"),
+    ((X, G, X, X), {"d_state": S}, "d_state"),
+    ((X, G, X, X), {"offsets": OFF, "d_state": S, "state": S[:1]}, "state"),
+])
+def test_gated_scan_grad(args, kw, error):
+    with pytest.raises((ValueError, TypeError), match=error):
+        gated.gated_scan_grad(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw,error", [
+    ((X, G), {}, "on the GPU"),
+    ((X, G, X), {}, "on the GPU"),
+    ((X, G, X[:3]), {}, "state"),
+    ((X, G), {"out_state": X.to(torch.bfloat16)}, "out_state"),
+    ((X, G, torch.zeros(10, 4).t()), {}, "contiguous"),
+    ((X, G), {"scale": None}, "scale"),
+])
+def test_gated_step(args, kw, error):
+    with pytest.raises((ValueError, TypeError), match=error):
+        gated.gated_step(*args, **kw)
+
+
+def test_step_into_a_shifted_view_of_the_state():
+    base = torch.zeros(5, 10)
+    with pytest.raises(ValueError, match="overlaps"):
+        gated.gated_step(X, G, base[:4], out_state=base[1:])
+
+
+def test_gated_entry_points_check_before_they_launch():
+    one, two = ctypes.c_void_p(256), ctypes.c_void_p(512)
+    lib = _capi.lib
+
+    def scan(dtype=0, gd=0, ld=10, la=5, rows=4, d=10, g=5, off=one, n=2, scale=0, s_in=None, s_out=one, out=one, lo=10):
+        return lib.ddm_gated_scan(one, dtype, ld, one, gd, la, rows, d, g, off, n, scale, s_in, s_out, out, lo, 1, None,
+                                  None, None, None)
+
+    def grad(h=one, ldh=10, lda=5, s0=two, ds=None):
+        return lib.ddm_gated_scan_grad(one, 0, 10, one, 0, 5, h, ldh, one, 10, 4, 10, 5, one, 2, 0, None, ds, s0, one, 10,
+                                       one, lda, 1, None, None, None, None)
+
+    def step(out=one, lo=10, d=10):
+        return lib.ddm_gated_step(one, 0, 10, one, 0, 5, 4, d, 5, 0, None, two, out, lo, None, None, None)
+    for call, cases in ((scan, (({"dtype": 5}, "types"), ({"dtype": 0, "gd": 1}, "types"), ({"dtype": 1, "gd": 2}, "types"),
+                                ({"g": 3}, "gates"), ({"g": 0}, "gates"), ({"ld": 9}, "strides"), ({"la": 4}, "strides"),
+                                ({"rows": -1}, "rows"), ({"n": -1}, "rows"), ({"scale": 3}, "scale"), ({"out": None}, "null"),
+                                ({"lo": 9}, "stride"), ({"off": None}, "one sequence"), ({"s_out": None}, "null"),
+                                ({"s_in": one}, "one buffer"), ({"rows": 1 << 39, "d": 1 << 20, "g": 1 << 20, "ld": 1 << 20,
+                                                                 "la": 1 << 20, "lo": 1 << 20}, "tiles"),
+                                ({"rows": 100000}, "scratch"))),
+                        (grad, (({"h": None}, "null"), ({"ldh": 9}, "stride"), ({"lda": 4}, "stride"),
+                                ({"s0": None}, "null"), ({"ds": two}, "one buffer"))),
+                        (step, (({"out": None}, "null"), ({"lo": 9}, "stride"), ({"d": 11}, "gates")))):
+        for kw, text in cases:
+            assert call(**kw) == _capi.DDM_E_ARG and text in last_error(), (kw, last_error())
+    assert lib.ddm_gated_scan_scratch_bytes(0, 8, 8, 0, 0) == 0
+    assert lib.ddm_gated_scan_scratch_bytes(100000, 8, 8, 0, 0) > 0
