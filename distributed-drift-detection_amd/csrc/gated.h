@@ -45,9 +45,32 @@ typedef type_of<float, DDM_F32> f32_t;
 typedef type_of<__bf16, DDM_BF16> bf16_t;
 typedef type_of<_Float16, DDM_F16> f16_t;
 
+// N entries of a row in as few registers as they have words; unpacked where they are used.
 template <typename T, int N>
-struct alignas(sizeof(typename T::E) * N) Raw {
-    typename T::E e[N];
+struct Raw {
+    static constexpr int kBytes = (int)sizeof(typename T::E) * N, kWords = (kBytes + 3) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const char* p) {
+        if (kBytes == 2)
+            w[0] = *(const uint16_t*)p;
+        else if (kBytes == 4)
+            w[0] = *(const uint32_t*)p;
+        else
+            *(uint2*)w = *(const uint2*)p;
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if (sizeof(typename T::E) == 4) return __uint_as_float(w[i]);
+        if (std::is_same<typename T::E, __bf16>::value) return __uint_as_float(i ? w[0] & 0xffff0000u : w[0] << 16);
+        const uint16_t h = (uint16_t)(i ? w[0] >> 16 : w[0]);
+        _Float16 f;
+        __builtin_memcpy(&f, &h, 2);
+        return (float)f;
+    }
+    // What was computed from it is not worth registers until it is used again.
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+    }
 };
 
 struct Args {
@@ -81,11 +104,10 @@ __device__ __forceinline__ Step after(const Step& p, const Step& q) {   // p, th
 __device__ __forceinline__ float apply(const Step& s, float h) { return s.a < 0.0f ? s.b : fmaf(s.a, h, s.b); }
 
 // ---- gates ---------------------------------------------------------------------------------------
-// 1 - e^y without cancellation: a series up to |y| = 0.7 (the first term left out is under 2^-27 of
-// the result), the difference beyond, where e^y is at most half.
-__device__ __forceinline__ float one_minus_exp(float y) {
-    float p = 2.7557319e-7f;                        // 1/10!
-    p = fmaf(p, y, 2.7557319e-6f);
+// 1 - e^y without cancellation, given e = e^y: a series up to |y| = 0.7 (the first term left out
+// is under 2^-26 of the result), the difference beyond, where e is at most half.
+__device__ __forceinline__ float one_minus_exp(float y, float e) {
+    float p = 2.7557319e-6f;                        // 1/9!
     p = fmaf(p, y, 2.4801587e-5f);
     p = fmaf(p, y, 1.9841270e-4f);
     p = fmaf(p, y, 1.3888889e-3f);
@@ -94,25 +116,39 @@ __device__ __forceinline__ float one_minus_exp(float y) {
     p = fmaf(p, y, 1.6666667e-1f);
     p = fmaf(p, y, 0.5f);
     p = fmaf(p, y, 1.0f);
-    return fabsf(y) <= 0.7f ? -y * p : 1.0f - __builtin_amdgcn_exp2f(y * 1.4426950408889634f);
+    return fabsf(y) <= 0.7f ? -y * p : 1.0f - e;
 }
-// e^l: the product's rounding, carried, keeps the exponential's error at its own.
-__device__ __forceinline__ float gate(float l) {
-    const float y = l * 1.4426950408889634f;
-    const float r = fmaf(l, 1.4426950408889634f, -y);
-    const float e = __builtin_amdgcn_exp2f(y);
-    return fabsf(y) < 126.0f ? fmaf(e * 0.6931471805599453f, r, e) : e;
+// a = e^l and the input's factor.  The exponential's argument is rounded once: half a step for each
+// binary order that a loses, which is less the less a weighs.
+struct Gate {
+    float a, f;
+};
+template <int SCALE>
+__device__ __forceinline__ Gate gate_of(float l) {
+    Gate g;
+    g.a = __builtin_amdgcn_exp2f(l * 1.4426950408889634f);
+    g.f = SCALE == DDM_GATED_NONE   ? 1.0f
+          : SCALE == DDM_GATED_EWMA ? one_minus_exp(l, g.a)
+                                    : __builtin_amdgcn_sqrtf(fmaxf(one_minus_exp(2.0f * l, g.a * g.a), 0.0f));
+    return g;
 }
-__device__ __forceinline__ float input_factor(float l, int scale) {
-    if (scale == DDM_GATED_NONE) return 1.0f;
-    if (scale == DDM_GATED_EWMA) return one_minus_exp(l);
-    return __builtin_amdgcn_sqrtf(fmaxf(one_minus_exp(2.0f * l), 0.0f));
+// The factor's derivative by l.
+template <int SCALE>
+__device__ __forceinline__ float slope_of(const Gate& g) {
+    if (SCALE == DDM_GATED_NONE) return 0.0f;
+    if (SCALE == DDM_GATED_EWMA) return -g.a;
+    // a^2 / f by the reciprocal of 1 step's error
+    return g.f > 0.0f ? -(g.a * g.a) * __builtin_amdgcn_rcpf(g.f) : g.f - g.f;        // NaN stays NaN
 }
-// ... and its derivative by l.
-__device__ __forceinline__ float input_slope(float a, float f, int scale) {
-    if (scale == DDM_GATED_NONE) return 0.0f;
-    if (scale == DDM_GATED_EWMA) return -a;
-    return f > 0.0f ? -(a * a) / f : f - f;        // NaN stays NaN
+// f(std::integral_constant<int, scale>()): one branch a tile, not one an entry.
+template <typename F>
+__device__ __forceinline__ void with_scale(int scale, F f) {
+    if (scale == DDM_GATED_NONE)
+        f(std::integral_constant<int, DDM_GATED_NONE>());
+    else if (scale == DDM_GATED_EWMA)
+        f(std::integral_constant<int, DDM_GATED_EWMA>());
+    else
+        f(std::integral_constant<int, DDM_GATED_UNIT>());
 }
 
 // ---- a tile's place -------------------------------------------------------------------------------
@@ -126,14 +162,27 @@ __device__ __forceinline__ Place take(const Args& a) {
     if (a.ticket) {
         if (threadIdx.x == 0) sh = atomicAdd(a.ticket, 1u);
         __syncthreads();
-        t = sh;
+        t = __builtin_amdgcn_readfirstlane(sh);      // the same in every lane, and known to be
     }
     return Place{(int64_t)(t / (uint32_t)a.ncb), (int)(t % (uint32_t)a.ncb)};
 }
 
-// Which rows of [row0, row0 + nrows) begin and end a sequence (its number, or -1).
-__device__ __forceinline__ void mark_rows(const Args& a, int64_t row0, int nrows, int32_t* begins, int32_t* ends) {
-    for (int i = threadIdx.x; i < nrows; i += NT) begins[i] = ends[i] = -1;
+// Which rows of a tile begin and end a sequence: a bit a row, and the sequence's number where it is set.
+struct Marks {
+    uint32_t *begin_bits, *end_bits;
+    int32_t *begins, *ends;
+    __device__ __forceinline__ Marks(int32_t* lds, int rows)
+        : begin_bits((uint32_t*)lds), end_bits((uint32_t*)lds + rows / 32), begins(lds + rows / 16),
+          ends(lds + rows / 16 + rows) {}
+    static constexpr int bytes(int rows) { return (rows / 16 + 2 * rows) * 4; }
+    // The lane's R rows from `at` on.
+    template <int R>
+    static __device__ __forceinline__ uint32_t lane(const uint32_t* bits, int at) {
+        return (bits[at >> 5] >> (at & 31)) & ((1u << R) - 1u);
+    }
+};
+__device__ __forceinline__ void mark_rows(const Args& a, int64_t row0, int nrows, const Marks& m) {
+    for (int i = threadIdx.x; i < nrows / 16; i += NT) m.begin_bits[i] = 0;     // and the end bits behind
     int64_t lo = 0, hi = a.n;                       // the first sequence that ends behind row0
     while (lo < hi) {
         const int64_t mid = (lo + hi) / 2;
@@ -147,10 +196,26 @@ __device__ __forceinline__ void mark_rows(const Args& a, int64_t row0, int nrows
         const int64_t b = a.off[s], e = a.off[s + 1];
         if (b >= row0 + nrows) break;
         if (e <= b) continue;
-        if (b >= row0) begins[b - row0] = (int32_t)s;
-        if (e > row0 && e <= row0 + nrows) ends[e - 1 - row0] = (int32_t)s;
+        if (b >= row0) {
+            const int i = (int)(b - row0);
+            m.begins[i] = (int32_t)s;
+            atomicOr(&m.begin_bits[i >> 5], 1u << (i & 31));
+        }
+        if (e > row0 && e <= row0 + nrows) {
+            const int i = (int)(e - 1 - row0);
+            m.ends[i] = (int32_t)s;
+            atomicOr(&m.end_bits[i >> 5], 1u << (i & 31));
+        }
     }
     __syncthreads();
+}
+// Bits of the R rows from r0 on that lie in [first, end).
+template <int R>
+__device__ __forceinline__ uint32_t rows_within(int64_t r0, int64_t first, int64_t end) {
+    const int64_t lo = first - r0, hi = end - r0;
+    const uint32_t upto = hi <= 0 ? 0u : hi >= R ? (1u << R) - 1u : (1u << (int)hi) - 1u;
+    const uint32_t before = lo <= 0 ? 0u : lo >= R ? (1u << R) - 1u : (1u << (int)lo) - 1u;
+    return upto & ~before;
 }
 
 // ---- the state before a lane's rows -----------------------------------------------------------------
@@ -159,12 +224,41 @@ struct ScanLds {
     float a[W][64 * VEC], b[W][64 * VEC];
 };
 
-// Steps of the workgroup's time groups composed in order, a channel apart: what is before the
-// lane's own, and all together.
+__device__ __forceinline__ uint64_t pack(float a, float b) {
+    const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    return w == kUnset ? w ^ 1u : w;               // two NaN of all ones: another NaN
+}
+__device__ __forceinline__ Step unpack(uint64_t w) {
+    return Step{__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
+}
+__device__ __forceinline__ void publish(uint64_t* p, uint64_t w) {
+    __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The first `count` (at most N) words of a column, all asked for at once; unset ones, if the guard
+// ever ran out, are NaN.
+template <int N>
+__device__ __forceinline__ void await(const uint64_t* p, int64_t stride, int count, uint64_t (&w)[N]) {
+    for (uint32_t spin = 0;; ++spin) {
+        bool set = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = i < count ? peek(p + i * stride) : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) set = set && w[i] != kUnset;
+        if (set || spin == kSpinLimit) return;
+        __builtin_amdgcn_s_sleep(1);
+    }
+}
+
+// From the steps of every lane's rows to the state before them: lanes of a wave by shuffles, the
+// waves and the tiles before by a thread for each channel.
 template <int VEC>
-__device__ __forceinline__ void block_scan(const Step (&own)[VEC], int cl, ScanLds<VEC>& l, Step (&before)[VEC],
-                                           Step (&all)[VEC]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ void chain(const Args& a, const Place& at, const Step (&own)[VEC], ScanLds<VEC>& l,
+                                      float (&h)[VEC]) {
+    const int cl = 1 << a.cl_bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int cols = cl * VEC, mine = (lane & (cl - 1)) * VEC;
     Step s[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) s[v] = own[v];
@@ -178,114 +272,76 @@ __device__ __forceinline__ void block_scan(const Step (&own)[VEC], int cl, ScanL
     if (lane >= 64 - cl) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            l.a[wave][(lane & (cl - 1)) * VEC + v] = s[v].a;
-            l.b[wave][(lane & (cl - 1)) * VEC + v] = s[v].b;
+            l.a[wave][mine + v] = s[v].a;
+            l.b[wave][mine + v] = s[v].b;
         }
     }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        s[v] = Step{__shfl_up(s[v].a, cl), __shfl_up(s[v].b, cl)};
-        if (lane < cl) s[v] = Step{1.0f, 0.0f};
-        all[v] = Step{1.0f, 0.0f};
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
+    if (cl < 64) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            if (w == wave) before[v] = after(all[v], s[v]);
-            const int c = (lane & (cl - 1)) * VEC + v;
-            all[v] = after(all[v], Step{l.a[w][c], l.b[w][c]});
+            s[v] = Step{__shfl_up(s[v].a, cl), __shfl_up(s[v].b, cl)};
+            if (lane < cl) s[v] = Step{1.0f, 0.0f};
         }
     }
     __syncthreads();
-}
-
-__device__ __forceinline__ uint64_t pack(float a, float b) {
-    const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-    return w == kUnset ? w ^ 1u : w;               // two NaN of all ones: another NaN
-}
-__device__ __forceinline__ void publish(uint64_t* p, uint64_t w) {
-    __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-template <int N>
-__device__ __forceinline__ void await(const uint64_t* p, uint64_t (&w)[N]) {
-    for (uint32_t spin = 0;; ++spin) {
-        bool set = true;
+    if ((int)threadIdx.x < cols) {
+        const int col = threadIdx.x;
+        Step all{1.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            w[i] = __hip_atomic_load(p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            set = set && w[i] != kUnset;
-        }
-        if (set || spin == kSpinLimit) return;      // unset words are NaN
-        __builtin_amdgcn_s_sleep(1);
-    }
-}
-
-// From the steps of every lane's rows to the state before them.
-template <int VEC>
-__device__ __forceinline__ void chain(const Args& a, const Place& at, const Step (&own)[VEC], ScanLds<VEC>& l,
-                                      float (&h)[VEC]) {
-    const int cl = 1 << a.cl_bits, tg = threadIdx.x >> a.cl_bits;
-    Step before[VEC], all[VEC];
-    block_scan<VEC>(own, cl, l, before, all);
-    float carry[VEC];
+        for (int w = 0; w < W; ++w) all = after(all, Step{l.a[w][col], l.b[w][col]});
+        float carry = 0.0f;
+        if (a.ticket) {
+            const int64_t c = (int64_t)at.block * cols + col, g = at.tile / a.group;
+            const int in_group = (int)(at.tile % a.group);
+            const bool last = in_group == a.group - 1, more = at.tile + 1 < a.ntiles;
+            if (!last && more) publish(a.agg + at.tile * a.dp + c, pack(all.a, all.b));
+            // the tiles before in the group first: they run beside this one; the group before is
+            // what there may be a wait for
+            Step sum{1.0f, 0.0f};
+            for (int j = 0; j < in_group; j += 8) {
+                uint64_t w[8];
+                await<8>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = 0.0f;
-    if (a.ticket) {
-        const int64_t c = ((int64_t)at.block * cl + (threadIdx.x & (cl - 1))) * VEC;
-        const int64_t g = at.tile / a.group;
-        const int in_group = (int)(at.tile % a.group);
-        const bool last = in_group == a.group - 1;
-        if (tg == 0 && !last && at.tile + 1 < a.ntiles) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) publish(a.agg + at.tile * a.dp + c + v, pack(all[v].a, all[v].b));
-        }
-        if (at.tile > 0) {
-            // time groups share the tiles before this one in the group; the first also takes the
-            // state before the group, a step that forgets everything
-            Step p[VEC], none[VEC], sum[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) p[v] = Step{1.0f, 0.0f};
-            uint64_t w[VEC];
-            if (tg == 0 && g > 0) {
-                await<VEC>(a.inc + (g - 1) * a.dp + c, w);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) p[v] = Step{kCut, __uint_as_float((uint32_t)w[v])};
+                for (int i = 0; i < 8; ++i)
+                    if (j + i < in_group) sum = after(sum, unpack(w[i]));
             }
-            const int per = (a.group + (NT >> a.cl_bits) - 1) / (NT >> a.cl_bits);
-            for (int i = 0; i < per; ++i) {
-                const int j = tg * per + i;
-                if (j < in_group) {
-                    await<VEC>(a.agg + (g * a.group + j) * a.dp + c, w);
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v)
-                        p[v] = after(p[v], Step{__uint_as_float((uint32_t)w[v]), __uint_as_float((uint32_t)(w[v] >> 32))});
-                }
+            if (g > 0) {
+                uint64_t w[1];
+                await<1>(a.inc + (g - 1) * a.dp + c, 0, 1, w);
+                carry = unpack(w[0]).a;
             }
-            block_scan<VEC>(p, cl, l, none, sum);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) carry[v] = apply(sum[v], 0.0f);
+            carry = apply(sum, carry);
+            if (last && more) publish(a.inc + g * a.dp + c, pack(apply(all, carry), 0.0f));
         }
-        if (tg == 0 && last && at.tile + 1 < a.ntiles) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) publish(a.inc + g * a.dp + c + v, pack(apply(all[v], carry[v]), 0.0f));
+        for (int w = 0; w < W; ++w) {
+            const float next = apply(Step{l.a[w][col], l.b[w][col]}, carry);
+            l.b[w][col] = carry;
+            carry = next;
         }
     }
+    __syncthreads();
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = apply(before[v], carry[v]);
+    for (int v = 0; v < VEC; ++v) {
+        h[v] = l.b[wave][mine + v];
+        if (cl < 64) h[v] = apply(s[v], h[v]);
+    }
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> load(const char* base, int64_t ld, int64_t row, int c) {
-    return *(const Raw<T, VEC>*)(base + row * ld + (int64_t)c * sizeof(typename T::E));
+    Raw<T, VEC> r;
+    r.load(base + row * ld + (int64_t)c * sizeof(typename T::E));
+    return r;
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store(char* base, int64_t ld, int64_t row, int c, const float (&f)[VEC]) {
-    Raw<T, VEC> r;
+    struct alignas(sizeof(typename T::E) * VEC) Out {
+        typename T::E e[VEC];
+    } o;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) r.e[v] = (typename T::E)f[v];
-    *(Raw<T, VEC>*)(base + row * ld + (int64_t)c * sizeof(typename T::E)) = r;
+    for (int v = 0; v < VEC; ++v) o.e[v] = (typename T::E)f[v];
+    *(Out*)(base + row * ld + (int64_t)c * sizeof(typename T::E)) = o;
 }
 // The gates of VEC channels: their own, or one that they share.
 template <typename L, int VEC, bool OWN>
@@ -294,7 +350,7 @@ struct Gates {
     __device__ __forceinline__ void load_row(const Args& a, int64_t row, int c) {
         r = load<L, OWN ? VEC : 1>(a.l, a.ld_l, row, OWN ? c : c / a.share);
     }
-    __device__ __forceinline__ float operator[](int v) const { return (float)r.e[OWN ? v : 0]; }
+    __device__ __forceinline__ float operator[](int v) const { return r[OWN ? v : 0]; }
 };
 
 // ---- launch shapes ---------------------------------------------------------------------------------
@@ -312,11 +368,11 @@ inline Shape shape_of(int64_t rows, int d, int share, int vec, bool grad) {
     s.ncb = (int)ceil_div(lanes, 1 << s.cl_bits);
     const int tg = NT >> s.cl_bits;
     // rows a lane: many, so that a tile's share of the chain is small, unless that leaves CUs idle
-    // or makes a tile's marks outgrow 16 KB of LDS
-    s.r = grad ? 8 : 16;
-    if (ceil_div(rows, tg * s.r) * s.ncb < 512 || tg * s.r > 2048) s.r = grad ? 2 : 4;
+    // or makes a tile's marks outgrow 34 KB of LDS
+    s.r = grad ? 8 : 16;                              // four operands a row, not two
+    if (ceil_div(rows, tg * s.r) * s.ncb < 512 || tg * s.r > 4096) s.r = 4;
     s.ntiles = ceil_div(rows, (int64_t)tg * s.r);
-    s.group = tg * 2 < 64 ? tg * 2 : 64;
+    s.group = s.cl_bits == 6 ? 16 : 64;              // what a tile reads of others stays under a tenth of its own
     s.dp = (int64_t)(s.ncb << s.cl_bits) * vec;
     s.dl_width = 1;
     s.dl_parts = 0;
@@ -332,37 +388,41 @@ inline Shape shape_of(int64_t rows, int d, int share, int vec, bool grad) {
 }
 
 inline int elem_size(int32_t dtype) { return dtype == DDM_F32 ? 4 : 2; }
-inline int wide_vec(int32_t dtype) { return 8 / elem_size(dtype); }
+inline int wide_vec(int32_t dtype) { return 4 / elem_size(dtype); }
 
-// 8 bytes of x a lane where every operand's rows are aligned for it and no such piece has two
-// gates; else an entry a lane.
+// 4 bytes of x a lane (and a row) where every operand's rows are aligned for it and no such piece
+// has two gates; else an entry a lane.  Wider pieces would leave fewer rows to a lane's registers,
+// and so make more tiles of the same rows.
 inline int vec_of(int32_t dtype, int32_t gate_dtype, int d, int share, std::initializer_list<const void*> x,
                   std::initializer_list<int64_t> ld, const void* l, int64_t ld_l, const void* dl, int64_t ld_dl) {
     const int v = wide_vec(dtype), es = elem_size(dtype), gs = elem_size(gate_dtype);
-    if (d % v || (share > 1 && share % v)) return 1;
+    if (v == 1 || d % v || (share > 1 && share % v)) return 1;
     for (const void* p : x)
-        if ((uintptr_t)p % 8) return 1;
+        if ((uintptr_t)p % 4) return 1;
     for (int64_t s : ld)
-        if (s * es % 8) return 1;
+        if (s * es % 4) return 1;
     if (share == 1 && ((uintptr_t)l % (v * gs) || ld_l * gs % (v * gs) || (uintptr_t)dl % (v * gs) || ld_dl * gs % (v * gs)))
         return 1;
     return v;
 }
 
-template <typename F>
-int with_types(int32_t dtype, int32_t gate_dtype, F f) {
-    if (dtype == DDM_F32) return f(f32_t(), f32_t());
-    if (dtype == DDM_BF16) return gate_dtype == DDM_F32 ? f(bf16_t(), f32_t()) : f(bf16_t(), bf16_t());
-    return gate_dtype == DDM_F32 ? f(f16_t(), f32_t()) : f(f16_t(), f16_t());
+// f(type of x, type of the gates, channels a lane, whether each has a gate of its own)
+template <typename X, typename L, typename F>
+void with_vec(int vec, bool own, F f) {
+    using one = std::integral_constant<int, 1>;
+    using two = std::integral_constant<int, 2>;
+    if (vec == 1) return f(X(), L(), one(), std::false_type());       // its index says which
+    if (sizeof(typename X::E) == 4) return;
+    using V = std::conditional_t<sizeof(typename X::E) == 4, one, two>;
+    if (own) return f(X(), L(), V(), std::true_type());
+    return f(X(), L(), V(), std::false_type());
 }
 template <typename F>
-void with_vec(int vec, bool own, F f) {
-    if (vec == 1) {
-        if (own) return f(std::integral_constant<int, 1>(), std::true_type());
-        return f(std::integral_constant<int, 1>(), std::false_type());
-    }
-    if (own) return f(std::integral_constant<int, 0>(), std::true_type());     // 0: the type's wide one
-    return f(std::integral_constant<int, 0>(), std::false_type());
+void with_types(int32_t dtype, int32_t gate_dtype, int vec, bool own, F f) {
+    if (dtype == DDM_F32) return with_vec<f32_t, f32_t>(vec, own, f);
+    if (dtype == DDM_BF16)
+        return gate_dtype == DDM_F32 ? with_vec<bf16_t, f32_t>(vec, own, f) : with_vec<bf16_t, bf16_t>(vec, own, f);
+    return gate_dtype == DDM_F32 ? with_vec<f16_t, f32_t>(vec, own, f) : with_vec<f16_t, f16_t>(vec, own, f);
 }
 
 inline int check(const char* who, int32_t dtype, int32_t gate_dtype, int64_t rows, int64_t d, int64_t gates,

@@ -4,9 +4,8 @@
 namespace ddm {
 namespace gated {
 
-// ---- forward ----------------------------------------------------------------------------------------
 template <typename X, typename L, int VEC, bool OWN, int R>
-__global__ __launch_bounds__(NT) void k_gated_scan(Args a) {
+__global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
     const Place at = take(a);
@@ -16,58 +15,93 @@ __global__ __launch_bounds__(NT) void k_gated_scan(Args a) {
     const bool active = c < a.d;
     Raw<X, VEC> x[R];
     Gates<L, VEC, OWN> l[R];
+    if (row0 + tr <= a.rows) {
+        if (active)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (active && r0 + r < a.rows) {
-            x[r] = load<X, VEC>(a.x, a.ld_x, r0 + r, c);
-            l[r].load_row(a, r0 + r, c);
-        }
+            for (int r = 0; r < R; ++r) {
+                x[r] = load<X, VEC>(a.x, a.ld_x, r0 + r, c);
+                l[r].load_row(a, r0 + r, c);
+            }
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (active && r0 + r < a.rows) {
+                x[r] = load<X, VEC>(a.x, a.ld_x, r0 + r, c);
+                l[r].load_row(a, r0 + r, c);
+            }
     }
-    int32_t *begins = marks, *ends = marks + tr;
-    int64_t first = 0, end = a.rows;
+    const Marks m(marks, tr);
+    uint32_t begins, ends, inside;
     if (a.off) {
-        mark_rows(a, row0, tr, begins, ends);
-        first = a.off[0];
-        end = a.off[a.n];
-        end = end < a.rows ? end : a.rows;
+        mark_rows(a, row0, tr, m);
+        begins = Marks::lane<R>(m.begin_bits, tg * R);
+        ends = Marks::lane<R>(m.end_bits, tg * R);
+        const int64_t end = a.off[a.n];
+        inside = rows_within<R>(r0, a.off[0], end < a.rows ? end : a.rows);
+    } else {
+        begins = r0 == 0;
+        ends = a.rows - 1 >= r0 && a.rows - 1 < r0 + R ? 1u << (int)(a.rows - 1 - r0) : 0u;
+        inside = rows_within<R>(r0, 0, a.rows);
     }
-    float b[R][VEC];
-    uint32_t cut = 0;                                // rows whose state before is no factor
+    begins &= inside;
+    ends &= inside;
+    const bool plain = !__any(active && (begins || ends || inside != (1u << R) - 1u));
+
+    float g[R][VEC], b[R][VEC];
     Step own[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
+    with_scale(a.scale, [&](auto scale) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t row = r0 + r;
-        const bool inside = active && row >= first && row < end;
-        const int s = !inside ? -1 : a.off ? begins[tg * R + r] : row == 0 ? 0 : -1;
-        if (!inside || s >= 0) cut |= 1u << r;
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float g = 0.0f, y = 0.0f;
-            if (inside) {
-                const float lv = l[r][v];
-                g = gate(lv);
-                y = input_factor(lv, a.scale) * (float)x[r].e[v];
-                if (s >= 0 && a.state_in) y = fmaf(g, a.state_in[(int64_t)s * a.d + c + v], y);
+            for (int v = 0; v < VEC; ++v) {
+                const Gate q = gate_of<scale()>(l[r][v]);
+                g[r][v] = q.a;
+                b[r][v] = q.f * x[r][v];
+                own[v].a *= q.a;
+                own[v].b = fmaf(q.a, own[v].b, b[r][v]);
             }
-            b[r][v] = y;
-            own[v] = after(own[v], Step{cut >> r & 1 ? kCut : g, y});
+    });
+    if (!plain) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool in = active && inside >> r & 1, first = begins >> r & 1;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if (in && first && a.state_in) {
+                    const int64_t s = a.off ? m.begins[tg * R + r] : 0;
+                    b[r][v] = fmaf(g[r][v], a.state_in[s * a.d + c + v], b[r][v]);
+                }
+                if (!in) b[r][v] = 0.0f;
+                if (!in || first) g[r][v] = kCut;
+                own[v] = after(own[v], Step{g[r][v], b[r][v]});
+            }
         }
     }
     float h[VEC];
     chain<VEC>(a, at, own, lds, h);
+    if (plain) {
+        if (!active) return;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) h[v] = fmaf(g[r][v], h[v], b[r][v]);
+            store<X, VEC>(a.out, a.ld_h, r0 + r, c, h);
+        }
+        return;
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t row = r0 + r;
-        const bool inside = active && row >= first && row < end;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = cut >> r & 1 ? b[r][v] : fmaf(gate(l[r][v]), h[v], b[r][v]);
-        if (inside || (a.fill && active && row < a.rows)) store<X, VEC>(a.out, a.ld_h, row, c, h);
-        const int s = !inside ? -1 : a.off ? ends[tg * R + r] : row == a.rows - 1 ? 0 : -1;
-        if (s >= 0) {
+        for (int v = 0; v < VEC; ++v) h[v] = apply(Step{g[r][v], b[r][v]}, h[v]);
+        if (active && (inside >> r & 1 || (a.fill && r0 + r < a.rows))) store<X, VEC>(a.out, a.ld_h, r0 + r, c, h);
+        if (active && ends >> r & 1) {
+            const int64_t s = a.off ? m.ends[tg * R + r] : 0;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) a.state_out[(int64_t)s * a.d + c + v] = h[v];
+            for (int v = 0; v < VEC; ++v) a.state_out[s * a.d + c + v] = h[v];
         }
     }
 }
@@ -96,10 +130,14 @@ __global__ __launch_bounds__(256) void k_gated_step(Args a) {
     l.load_row(a, row, c);
     float h[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        const float before = a.state_in ? a.state_in[row * a.d + c + v] : 0.0f;
-        h[v] = fmaf(gate(l[v]), before, input_factor(l[v], a.scale) * (float)x.e[v]);
-    }
+    for (int v = 0; v < VEC; ++v) h[v] = a.state_in ? a.state_in[row * a.d + c + v] : 0.0f;
+    with_scale(a.scale, [&](auto scale) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const Gate q = gate_of<scale()>(l[v]);
+            h[v] = fmaf(q.a, h[v], q.f * x[v]);
+        }
+    });
 #pragma unroll
     for (int v = 0; v < VEC; ++v) a.state_out[row * a.d + c + v] = h[v];
     store<X, VEC>(a.out, a.ld_h, row, c, h);
@@ -186,20 +224,17 @@ extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const 
         a.state_out = state_out;
         if (int rc = begin(a, s, scratch, state_in, state_out, n * d, st)) return rc;
         if (rows == 0) return 0;
-        const size_t lds = offsets ? (size_t)(NT >> s.cl_bits) * s.r * 8 : 0;
-        return with_types(dtype, gate_dtype, [&](auto xt, auto lt) {
+        const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
+        const dim3 grid((unsigned)(s.ntiles * s.ncb));
+        with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
             using X = decltype(xt);
             using L = decltype(lt);
-            with_vec(vec, share == 1, [&](auto v, auto own) {
-                constexpr int V = v() ? 1 : 8 / (int)sizeof(typename X::E);
-                const dim3 grid((unsigned)(s.ntiles * s.ncb));
-                if (s.r == 16)
-                    k_gated_scan<X, L, V, own(), 16><<<grid, NT, lds, st>>>(a);
-                else
-                    k_gated_scan<X, L, V, own(), 4><<<grid, NT, lds, st>>>(a);
-            });
-            return launch_status("ddm_gated_scan");
+            if (s.r == 16)
+                k_gated_scan<X, L, v(), own(), 16><<<grid, NT, lds, st>>>(a);
+            else
+                k_gated_scan<X, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
         });
+        return launch_status("ddm_gated_scan");
     });
 }
 
@@ -235,14 +270,9 @@ extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const 
         a.scale = scale;
         a.state_in = state_in;
         a.state_out = state_out;
-        return with_types(dtype, gate_dtype, [&](auto xt, auto lt) {
-            using X = decltype(xt);
-            using L = decltype(lt);
-            with_vec(vec, share == 1, [&](auto v, auto own) {
-                constexpr int V = v() ? 1 : 8 / (int)sizeof(typename X::E);
-                k_gated_step<X, L, V, own()><<<dim3((unsigned)blocks), 256, 0, st>>>(a);
-            });
-            return launch_status("ddm_gated_step");
+        with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
+            k_gated_step<decltype(xt), decltype(lt), v(), own()><<<dim3((unsigned)blocks), 256, 0, st>>>(a);
         });
+        return launch_status("ddm_gated_step");
     });
 }

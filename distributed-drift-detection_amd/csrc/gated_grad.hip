@@ -4,102 +4,138 @@
 namespace ddm {
 namespace gated {
 
-// ---- gradient ----------------------------------------------------------------------------------------
-// Rows in the opposite order: position p of the recurrence is row ntiles * tr - 1 - p.
+// Rows in the opposite order: position p of the recurrence is row ntiles * tr - 1 - p, and a lane's
+// rows run from its last one back; bits of rows count from the first, as in the forward.
 template <typename X, typename L, int VEC, bool OWN, int R>
-__global__ __launch_bounds__(NT) void k_gated_grad(Args a) {
+__global__ __launch_bounds__(NT, 4) void k_gated_grad(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
     const Place at = take(a);
-    const int cl = 1 << a.cl_bits, tg = threadIdx.x >> a.cl_bits, tr = (NT >> a.cl_bits) * R;
+    const int cl = 1 << a.cl_bits, tg = (NT >> a.cl_bits) - 1 - (threadIdx.x >> a.cl_bits);
+    const int tr = (NT >> a.cl_bits) * R;
     const int c = (at.block * cl + (int)(threadIdx.x & (cl - 1))) * VEC;
-    const int64_t row0 = (a.ntiles - 1 - at.tile) * tr, top = row0 + tr - 1 - tg * R;    // the lane's last row
+    const int64_t row0 = (a.ntiles - 1 - at.tile) * tr, r0 = row0 + tg * R;
     const bool active = c < a.d;
     Raw<X, VEC> x[R], dh[R], hp[R];
     Gates<L, VEC, OWN> l[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t row = top - r;
+        const int64_t row = r0 + r;
         if (active && row < a.rows) {
-            x[r] = load<X, VEC>(a.x, a.ld_x, row, c);
-            l[r].load_row(a, row, c);
             dh[r] = load<X, VEC>(a.dh, a.ld_dh, row, c);
+            l[r].load_row(a, row, c);
+            x[r] = load<X, VEC>(a.x, a.ld_x, row, c);
             if (row > 0) hp[r] = load<X, VEC>(a.h, a.ld_h, row - 1, c);
         }
     }
-    int32_t *begins = marks, *ends = marks + tr;
-    int64_t first = 0, end = a.rows;
+    const Marks m(marks, tr);
+    uint32_t begins, ends, inside;
     if (a.off) {
-        mark_rows(a, row0, tr, begins, ends);
-        first = a.off[0];
-        end = a.off[a.n];
-        end = end < a.rows ? end : a.rows;
+        mark_rows(a, row0, tr, m);
+        begins = Marks::lane<R>(m.begin_bits, tg * R);
+        ends = Marks::lane<R>(m.end_bits, tg * R);
+        const int64_t end = a.off[a.n];
+        inside = rows_within<R>(r0, a.off[0], end < a.rows ? end : a.rows);
+    } else {
+        begins = r0 == 0;
+        ends = a.rows - 1 >= r0 && a.rows - 1 < r0 + R ? 1u << (int)(a.rows - 1 - r0) : 0u;
+        inside = rows_within<R>(r0, 0, a.rows);
     }
-    auto inside = [&](int64_t row) { return active && row >= first && row < end; };
-    auto ends_at = [&](int64_t row) { return a.off ? ends[row - row0] : row == a.rows - 1 ? 0 : -1; };
-    auto given = [&](int s, int v) { return a.dstate ? a.dstate[(int64_t)s * a.d + c + v] : 0.0f; };
+    begins &= inside;
+    ends &= inside;
+    const bool plain = !__any(active && (begins || ends || inside != (1u << R) - 1u));
+    auto given = [&](int r, int v) {
+        const int64_t s = a.off ? m.ends[tg * R + r] : 0;
+        return a.dstate ? a.dstate[s * a.d + c + v] : 0.0f;
+    };
+
     Step own[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t row = top - r;
-        const bool in = inside(row);
-        const int s = in ? ends_at(row) : -1;
+    for (int r = R - 1; r >= 0; --r)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            Step q{kCut, 0.0f};
-            if (in) {
-                const float g = gate(l[r][v]), y = (float)dh[r].e[v];
-                q = s >= 0 ? Step{kCut, g * (y + given(s, v))} : Step{g, g * y};
-            }
-            own[v] = after(own[v], q);
-        }
-    }
-    float u[VEC];
-    chain<VEC>(a, at, own, lds, u);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t row = top - r;
-        const bool in = inside(row), put = in || (a.fill && active && row < a.rows);
-        const int s_end = in ? ends_at(row) : -1;
-        const int s_begin = !in ? -1 : a.off ? begins[row - row0] : row == 0 ? 0 : -1;
-        float dx[VEC], dl[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            dx[v] = dl[v] = 0.0f;
-            if (in) {
-                const float lv = l[r][v], g = gate(lv), f = input_factor(lv, a.scale);
-                const float grad = (float)dh[r].e[v] + (s_end >= 0 ? given(s_end, v) : u[v]);
-                const float before = s_begin < 0 ? (float)hp[r].e[v]
-                                     : a.state_in ? a.state_in[(int64_t)s_begin * a.d + c + v] : 0.0f;
-                dx[v] = grad * f;
-                dl[v] = grad * fmaf(input_slope(g, f, a.scale), (float)x[r].e[v], g * before);
-                u[v] = g * grad;
-                if (s_begin >= 0) a.state_out[(int64_t)s_begin * a.d + c + v] = u[v];
+            const float g = gate_of<DDM_GATED_NONE>(l[r][v]).a, y = dh[r][v];
+            if (plain) {
+                own[v].a *= g;
+                own[v].b = g * (own[v].b + y);
             } else {
-                u[v] = 0.0f;
+                Step q{kCut, 0.0f};
+                if (active && inside >> r & 1)
+                    q = ends >> r & 1 ? Step{kCut, g * (y + given(r, v))} : Step{g, g * y};
+                own[v] = after(own[v], q);
             }
         }
-        if (put) store<X, VEC>(a.dx, a.ld_dx, row, c, dx);
-        if (OWN) {
-            if (put) store<L, VEC>(a.dl, a.ld_dl, row, c, dl);
-        } else {
-            float sum = dl[0];
+    float u[VEC];
 #pragma unroll
-            for (int v = 1; v < VEC; ++v) sum += dl[v];
-            for (int k = 1; k < a.dl_width; k <<= 1) sum += __shfl_xor(sum, k);
-            if (put && (threadIdx.x & (a.dl_width - 1)) == 0) {
-                if (a.dl_part) {
-                    const int64_t parts = a.d / (VEC * a.dl_width);
-                    a.dl_part[row * parts + c / (VEC * a.dl_width)] = sum;
-                } else {
-                    *(typename L::E*)(a.dl + row * a.ld_dl + (int64_t)(c / a.share) * sizeof(typename L::E)) =
-                        (typename L::E)sum;
-                }
-            }
-        }
+    for (int r = 0; r < R; ++r) {
+        dh[r].forget();
+        l[r].r.forget();
     }
+    chain<VEC>(a, at, own, lds, u);
+    auto put = [&](int r, const float (&dx)[VEC], const float (&dl)[VEC], bool here) {
+        const int64_t row = r0 + r;
+        if (here) store<X, VEC>(a.dx, a.ld_dx, row, c, dx);
+        if (OWN) {
+            if (here) store<L, VEC>(a.dl, a.ld_dl, row, c, dl);
+            return;
+        }
+        float sum = dl[0];
+#pragma unroll
+        for (int v = 1; v < VEC; ++v) sum += dl[v];
+        for (int k = 1; k < a.dl_width; k <<= 1) sum += __shfl_xor(sum, k);
+        if (here && (threadIdx.x & (a.dl_width - 1)) == 0) {
+            if (a.dl_part)
+                a.dl_part[row * (a.d / (VEC * a.dl_width)) + c / (VEC * a.dl_width)] = sum;
+            else
+                *(typename L::E*)(a.dl + row * a.ld_dl + (int64_t)(c / a.share) * sizeof(typename L::E)) =
+                    (typename L::E)sum;
+        }
+    };
+    with_scale(a.scale, [&](auto scale) {
+        if (plain) {
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r) {
+                float dx[VEC], dl[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const Gate q = gate_of<scale()>(l[r][v]);
+                    const float grad = dh[r][v] + u[v];
+                    dx[v] = grad * q.f;
+                    dl[v] = grad * fmaf(slope_of<scale()>(q), x[r][v], q.a * hp[r][v]);
+                    u[v] = q.a * grad;
+                }
+                put(r, dx, dl, active);
+            }
+            return;
+        }
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r) {
+            const bool in = active && inside >> r & 1;
+            float dx[VEC], dl[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                dx[v] = dl[v] = 0.0f;
+                if (!in) {
+                    u[v] = 0.0f;
+                    continue;
+                }
+                const Gate q = gate_of<scale()>(l[r][v]);
+                const float grad = dh[r][v] + (ends >> r & 1 ? given(r, v) : u[v]);
+                float before = hp[r][v];
+                u[v] = q.a * grad;
+                if (begins >> r & 1) {
+                    const int64_t s = a.off ? m.begins[tg * R + r] : 0;
+                    before = a.state_in ? a.state_in[s * a.d + c + v] : 0.0f;
+                    a.state_out[s * a.d + c + v] = u[v];
+                }
+                dx[v] = grad * q.f;
+                dl[v] = grad * fmaf(slope_of<scale()>(q), x[r][v], q.a * before);
+            }
+            put(r, dx, dl, in || (a.fill && active && r0 + r < a.rows));
+        }
+    });
 }
 
 // Gates shared by more channels than a wave sums: the parts of each, in order.
@@ -173,28 +209,24 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
         a.state_out = d_state_in;
         if (int rc = begin(a, s, scratch, d_state_out, d_state_in, n * d, st)) return rc;
         if (rows == 0) return 0;
-        const size_t lds = offsets ? (size_t)(NT >> s.cl_bits) * s.r * 8 : 0;
-        return with_types(dtype, gate_dtype, [&](auto xt, auto lt) {
+        const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
+        const dim3 grid((unsigned)(s.ntiles * s.ncb));
+        const int64_t sums = ceil_div(rows * gates, 256);
+        if (s.dl_parts && sums > INT32_MAX) {
+            set_error("ddm_gated_scan_grad: %lld gate gradients", (long long)(rows * gates));
+            return DDM_E_ARG;
+        }
+        int rc = 0;
+        with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
             using X = decltype(xt);
             using L = decltype(lt);
-            with_vec(vec, share == 1, [&](auto v, auto own) {
-                constexpr int V = v() ? 1 : 8 / (int)sizeof(typename X::E);
-                const dim3 grid((unsigned)(s.ntiles * s.ncb));
-                if (s.r == 8)
-                    k_gated_grad<X, L, V, own(), 8><<<grid, NT, lds, st>>>(a);
-                else
-                    k_gated_grad<X, L, V, own(), 2><<<grid, NT, lds, st>>>(a);
-            });
-            if (int rc = launch_status("ddm_gated_scan_grad")) return rc;
-            if (s.dl_parts) {
-                const int64_t blocks = ceil_div(rows * gates, 256);
-                if (blocks > INT32_MAX) {
-                    set_error("ddm_gated_scan_grad: %lld gate gradients", (long long)(rows * gates));
-                    return DDM_E_ARG;
-                }
-                k_gated_sum<L><<<dim3((unsigned)blocks), 256, 0, st>>>(a, gates, s.dl_parts);
-            }
-            return launch_status("ddm_gated_scan_grad");
+            if (s.r == 8)
+                k_gated_grad<X, L, v(), own(), 8><<<grid, NT, lds, st>>>(a);
+            else
+                k_gated_grad<X, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
+            rc = launch_status("ddm_gated_scan_grad");
+            if (!rc && s.dl_parts) k_gated_sum<L><<<dim3((unsigned)sums), 256, 0, st>>>(a, gates, s.dl_parts);
         });
+        return rc ? rc : launch_status("ddm_gated_scan_grad");
     });
 }
