@@ -328,28 +328,31 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
     }
 }
 
+// A lane's entries of a row: the row's address is the same in all lanes, and each lane's offset from
+// it the same in all rows (one register; check_tile keeps it under 2^31).
 template <typename T, int VEC>
-__device__ __forceinline__ Raw<T, VEC> load(const char* base, int64_t ld, int64_t row, int c) {
+__device__ __forceinline__ Raw<T, VEC> load(const char* row, uint32_t offset) {
     Raw<T, VEC> r;
-    r.load(base + row * ld + (int64_t)c * sizeof(typename T::E));
+    r.load(row + offset);
     return r;
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void store(char* base, int64_t ld, int64_t row, int c, const float (&f)[VEC]) {
+__device__ __forceinline__ void store(char* row, uint32_t offset, const float (&f)[VEC]) {
     struct alignas(sizeof(typename T::E) * VEC) Out {
         typename T::E e[VEC];
     } o;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) o.e[v] = (typename T::E)f[v];
-    *(Out*)(base + row * ld + (int64_t)c * sizeof(typename T::E)) = o;
+    *(Out*)(row + offset) = o;
 }
 // The gates of VEC channels: their own, or one that they share.
 template <typename L, int VEC, bool OWN>
 struct Gates {
     Raw<L, OWN ? VEC : 1> r;
-    __device__ __forceinline__ void load_row(const Args& a, int64_t row, int c) {
-        r = load<L, OWN ? VEC : 1>(a.l, a.ld_l, row, OWN ? c : c / a.share);
+    static __device__ __forceinline__ uint32_t column(const Args& a, int c) {
+        return (uint32_t)((OWN ? c : c / a.share) * (int)sizeof(typename L::E));
     }
+    __device__ __forceinline__ void load_row(const char* row, uint32_t offset) { r = load<L, OWN ? VEC : 1>(row, offset); }
     __device__ __forceinline__ float operator[](int v) const { return r[OWN ? v : 0]; }
 };
 
@@ -409,13 +412,12 @@ inline int vec_of(int32_t dtype, int32_t gate_dtype, int d, int share, std::init
 // f(type of x, type of the gates, channels a lane, whether each has a gate of its own)
 template <typename X, typename L, typename F>
 void with_vec(int vec, bool own, F f) {
-    using one = std::integral_constant<int, 1>;
-    using two = std::integral_constant<int, 2>;
-    if (vec == 1) return f(X(), L(), one(), std::false_type());       // its index says which
-    if (sizeof(typename X::E) == 4) return;
-    using V = std::conditional_t<sizeof(typename X::E) == 4, one, two>;
-    if (own) return f(X(), L(), V(), std::true_type());
-    return f(X(), L(), V(), std::false_type());
+    if constexpr (sizeof(typename X::E) == 2) {
+        using two = std::integral_constant<int, 2>;
+        if (vec == 2 && own) return f(X(), L(), two(), std::true_type());
+        if (vec == 2) return f(X(), L(), two(), std::false_type());
+    }
+    f(X(), L(), std::integral_constant<int, 1>(), std::false_type());      // its gate by its index
 }
 template <typename F>
 void with_types(int32_t dtype, int32_t gate_dtype, int vec, bool own, F f) {
@@ -441,11 +443,19 @@ inline int check(const char* who, int32_t dtype, int32_t gate_dtype, int64_t row
     return DDM_E_ARG;
 }
 
-// 0, or DDM_E_ARG where the grid has no room for the tiles.
-inline int check_grid(const char* who, const Shape& s) {
-    if (s.ntiles * s.ncb <= INT32_MAX) return 0;
-    set_error("%s: %lld tiles of %d channel blocks", who, (long long)s.ntiles, s.ncb);
-    return DDM_E_ARG;
+// 0, or DDM_E_ARG where the grid has no room for the tiles, or a tile's rows lie too far apart for 32 bits.
+inline int check_tile(const char* who, const Shape& s, std::initializer_list<int64_t> ld_bytes) {
+    if (s.ntiles * s.ncb > INT32_MAX) {
+        set_error("%s: %lld tiles of %d channel blocks", who, (long long)s.ntiles, s.ncb);
+        return DDM_E_ARG;
+    }
+    const int64_t rows = (int64_t)(NT >> s.cl_bits) * s.r;
+    for (int64_t ld : ld_bytes)
+        if (ld > (((int64_t)1 << 31) - (4 << 20)) / rows) {
+            set_error("%s: a row stride of %lld bytes (at most 2^31 / %lld)", who, (long long)ld, (long long)rows);
+            return DDM_E_ARG;
+        }
+    return 0;
 }
 
 inline int64_t scratch_bytes(const Shape& s, int64_t rows, int d) {

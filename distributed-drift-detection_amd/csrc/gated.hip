@@ -15,19 +15,24 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     const bool active = c < a.d;
     Raw<X, VEC> x[R];
     Gates<L, VEC, OWN> l[R];
+    const uint32_t lane_x = tg * R * (uint32_t)a.ld_x + c * (uint32_t)sizeof(typename X::E);
+    const uint32_t lane_h = tg * R * (uint32_t)a.ld_h + c * (uint32_t)sizeof(typename X::E);
+    const uint32_t lane_l = tg * R * (uint32_t)a.ld_l + Gates<L, VEC, OWN>::column(a, c);
+    const char *x0 = a.x + row0 * a.ld_x, *l0 = a.l + row0 * a.ld_l;
+    char* h0 = a.out + row0 * a.ld_h;
     if (row0 + tr <= a.rows) {
         if (active)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                x[r] = load<X, VEC>(a.x, a.ld_x, r0 + r, c);
-                l[r].load_row(a, r0 + r, c);
+                x[r] = load<X, VEC>(x0 + r * a.ld_x, lane_x);
+                l[r].load_row(l0 + r * a.ld_l, lane_l);
             }
     } else {
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (active && r0 + r < a.rows) {
-                x[r] = load<X, VEC>(a.x, a.ld_x, r0 + r, c);
-                l[r].load_row(a, r0 + r, c);
+                x[r] = load<X, VEC>(x0 + r * a.ld_x, lane_x);
+                l[r].load_row(l0 + r * a.ld_l, lane_l);
             }
     }
     const Marks m(marks, tr);
@@ -47,21 +52,28 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     ends &= inside;
     const bool plain = !__any(active && (begins || ends || inside != (1u << R) - 1u));
 
-    float g[R][VEC], b[R][VEC];
+    constexpr int G = OWN ? VEC : 1;                 // gates a lane; a cut is one of all its channels
+    float g[R][G], b[R][VEC];
     Step own[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
     with_scale(a.scale, [&](auto scale) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            float in[G];
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+                const Gate q = gate_of<scale()>(l[r][k]);
+                g[r][k] = q.a;
+                in[k] = q.f;
+            }
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const Gate q = gate_of<scale()>(l[r][v]);
-                g[r][v] = q.a;
-                b[r][v] = q.f * x[r][v];
-                own[v].a *= q.a;
-                own[v].b = fmaf(q.a, own[v].b, b[r][v]);
+                b[r][v] = in[v % G] * x[r][v];
+                own[v].a *= g[r][v % G];
+                own[v].b = fmaf(g[r][v % G], own[v].b, b[r][v]);
             }
+        }
     });
     if (!plain) {
 #pragma unroll
@@ -73,12 +85,15 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
             for (int v = 0; v < VEC; ++v) {
                 if (in && first && a.state_in) {
                     const int64_t s = a.off ? m.begins[tg * R + r] : 0;
-                    b[r][v] = fmaf(g[r][v], a.state_in[s * a.d + c + v], b[r][v]);
+                    b[r][v] = fmaf(g[r][v % G], a.state_in[s * a.d + c + v], b[r][v]);
                 }
                 if (!in) b[r][v] = 0.0f;
-                if (!in || first) g[r][v] = kCut;
-                own[v] = after(own[v], Step{g[r][v], b[r][v]});
             }
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+                if (!in || first) g[r][k] = kCut;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) own[v] = after(own[v], Step{g[r][v % G], b[r][v]});
         }
     }
     float h[VEC];
@@ -88,16 +103,16 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = fmaf(g[r][v], h[v], b[r][v]);
-            store<X, VEC>(a.out, a.ld_h, r0 + r, c, h);
+            for (int v = 0; v < VEC; ++v) h[v] = fmaf(g[r][v % G], h[v], b[r][v]);
+            store<X, VEC>(h0 + r * a.ld_h, lane_h, h);
         }
         return;
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = apply(Step{g[r][v], b[r][v]}, h[v]);
-        if (active && (inside >> r & 1 || (a.fill && r0 + r < a.rows))) store<X, VEC>(a.out, a.ld_h, r0 + r, c, h);
+        for (int v = 0; v < VEC; ++v) h[v] = apply(Step{g[r][v % G], b[r][v]}, h[v]);
+        if (active && (inside >> r & 1 || (a.fill && r0 + r < a.rows))) store<X, VEC>(h0 + r * a.ld_h, lane_h, h);
         if (active && ends >> r & 1) {
             const int64_t s = a.off ? m.ends[tg * R + r] : 0;
 #pragma unroll
@@ -125,9 +140,9 @@ __global__ __launch_bounds__(256) void k_gated_step(Args a) {
     const int64_t row = i / per;
     const int c = (int)(i % per) * VEC;
     if (row >= a.rows) return;
-    const Raw<X, VEC> x = load<X, VEC>(a.x, a.ld_x, row, c);
+    const Raw<X, VEC> x = load<X, VEC>(a.x + row * a.ld_x, c * (uint32_t)sizeof(typename X::E));
     Gates<L, VEC, OWN> l;
-    l.load_row(a, row, c);
+    l.load_row(a.l + row * a.ld_l, Gates<L, VEC, OWN>::column(a, c));
     float h[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) h[v] = a.state_in ? a.state_in[row * a.d + c + v] : 0.0f;
@@ -140,7 +155,7 @@ __global__ __launch_bounds__(256) void k_gated_step(Args a) {
     });
 #pragma unroll
     for (int v = 0; v < VEC; ++v) a.state_out[row * a.d + c + v] = h[v];
-    store<X, VEC>(a.out, a.ld_h, row, c, h);
+    store<X, VEC>(a.out + row * a.ld_h, c * (uint32_t)sizeof(typename X::E), h);
 }
 
 // The chain's buffers, the copy of the states, and where both are needed their launch.
@@ -199,7 +214,7 @@ extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const 
     const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype);
     const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
     const Shape s = shape_of(rows, (int)d, share, vec, false);
-    if (int rc = check_grid("ddm_gated_scan", s)) return rc;
+    if (int rc = check_tile("ddm_gated_scan", s, {ld_x * es, ld_a * gs, ld_out * es})) return rc;
     if (scratch_bytes(s, rows, (int)d) && !scratch) {
         set_error("ddm_gated_scan: invalid argument (no scratch)");
         return DDM_E_ARG;

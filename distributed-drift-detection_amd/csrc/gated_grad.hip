@@ -18,15 +18,24 @@ __global__ __launch_bounds__(NT, 4) void k_gated_grad(Args a) {
     const bool active = c < a.d;
     Raw<X, VEC> x[R], dh[R], hp[R];
     Gates<L, VEC, OWN> l[R];
+    auto lane_of = [&](int64_t ld) { return tg * R * (uint32_t)ld + c * (uint32_t)sizeof(typename X::E); };
+    const uint32_t lane_x = lane_of(a.ld_x), lane_h = lane_of(a.ld_h), lane_dh = lane_of(a.ld_dh);
+    const uint32_t column_l = Gates<L, VEC, OWN>::column(a, c), lane_l = tg * R * (uint32_t)a.ld_l + column_l;
+    auto load_row = [&](int r) {
+        const int64_t row = row0 + r;                 // of the first time group
+        dh[r] = load<X, VEC>(a.dh + row * a.ld_dh, lane_dh);
+        l[r].load_row(a.l + row * a.ld_l, lane_l);
+        x[r] = load<X, VEC>(a.x + row * a.ld_x, lane_x);
+        if (r0 + r > 0) hp[r] = load<X, VEC>(a.h + (row - 1) * a.ld_h, lane_h);
+    };
+    if (row0 + tr <= a.rows) {
+        if (active)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t row = r0 + r;
-        if (active && row < a.rows) {
-            dh[r] = load<X, VEC>(a.dh, a.ld_dh, row, c);
-            l[r].load_row(a, row, c);
-            x[r] = load<X, VEC>(a.x, a.ld_x, row, c);
-            if (row > 0) hp[r] = load<X, VEC>(a.h, a.ld_h, row - 1, c);
-        }
+            for (int r = 0; r < R; ++r) load_row(r);
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (active && r0 + r < a.rows) load_row(r);
     }
     const Marks m(marks, tr);
     uint32_t begins, ends, inside;
@@ -76,9 +85,9 @@ __global__ __launch_bounds__(NT, 4) void k_gated_grad(Args a) {
     chain<VEC>(a, at, own, lds, u);
     auto put = [&](int r, const float (&dx)[VEC], const float (&dl)[VEC], bool here) {
         const int64_t row = r0 + r;
-        if (here) store<X, VEC>(a.dx, a.ld_dx, row, c, dx);
+        if (here) store<X, VEC>(a.dx + (row0 + r) * a.ld_dx, lane_of(a.ld_dx), dx);
         if (OWN) {
-            if (here) store<L, VEC>(a.dl, a.ld_dl, row, c, dl);
+            if (here) store<L, VEC>(a.dl + (row0 + r) * a.ld_dl, tg * R * (uint32_t)a.ld_dl + column_l, dl);
             return;
         }
         float sum = dl[0];
@@ -89,8 +98,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_grad(Args a) {
             if (a.dl_part)
                 a.dl_part[row * (a.d / (VEC * a.dl_width)) + c / (VEC * a.dl_width)] = sum;
             else
-                *(typename L::E*)(a.dl + row * a.ld_dl + (int64_t)(c / a.share) * sizeof(typename L::E)) =
-                    (typename L::E)sum;
+                *(typename L::E*)(a.dl + row * a.ld_dl + column_l) = (typename L::E)sum;
         }
     };
     with_scale(a.scale, [&](auto scale) {
@@ -177,7 +185,9 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
     const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, h, d_h, d_x}, {ld_x, ld_h, ld_dh, ld_dx}, log_a, ld_a,
                            d_log_a, ld_da);
     const Shape s = shape_of(rows, (int)d, share, vec, true);
-    if (int rc = check_grid("ddm_gated_scan_grad", s)) return rc;
+    if (int rc = check_tile("ddm_gated_scan_grad", s,
+                            {ld_x * es, ld_a * gs, ld_h * es, ld_dh * es, ld_dx * es, ld_da * gs}))
+        return rc;
     if (scratch_bytes(s, rows, (int)d) && !scratch) {
         set_error("ddm_gated_scan_grad: invalid argument (no scratch)");
         return DDM_E_ARG;
