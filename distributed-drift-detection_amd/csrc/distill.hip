@@ -138,7 +138,7 @@ __device__ __forceinline__ void mark_kept(uint32_t* bits, bool set, int vector, 
 // The running maximum and sum of a part, kept columns apart.
 template <typename T, int NT, int NV>
 __device__ __forceinline__ Part sum_part(const uint4 (&raw)[NV], float c, bool rest, const uint32_t* bits) {
-    Part p = no_part();
+    Lane l = no_lane();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float f[T::kVec];
@@ -150,25 +150,9 @@ __device__ __forceinline__ Part sum_part(const uint4 (&raw)[NV], float c, bool r
                 for (int e = 0; e < T::kVec; ++e) f[e] = b >> e & 1 ? -INFINITY : f[e];
             }
         }
-        float m = f[0];
-#pragma unroll
-        for (int e = 1; e < T::kVec; ++e) m = fmaxf(m, f[e]);
-        if (__any(m > p.m)) rebase(p, fmaxf(p.m, m), c);
-#pragma unroll
-        for (int e = 0; e < T::kVec; ++e) p.s += __builtin_amdgcn_exp2f((f[e] - p.m) * c);
+        add_vector<false>(l, f, largest(f), c);
     }
-    return p;
-}
-
-template <int NT>
-__device__ __forceinline__ Part block_merge(Part p, float c, Part* sh) {
-    constexpr int W = NT / 64;
-    p = wave_merge(p, c);
-    if (W == 1) return p;
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = p;
-    __syncthreads();
-    const int lane = threadIdx.x & 63;
-    return wave_merge(lane < W ? sh[lane] : no_part(), c);
+    return part_of(l, c);
 }
 
 template <typename T>
@@ -279,9 +263,8 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs a) {
 
 // A workgroup a row while it fits and there are rows enough to give every CU one or two, or
 // nothing is gained by cutting it; parts as for the scores otherwise.
-inline Shape distill_shape(int64_t n, int64_t v, int vec, bool grad) {
-    const int64_t nvec = ceil_div(v + vec - 1, vec);
-    Shape s{256, 8, 1};
+inline Shape distill_shape(int64_t n, int64_t nvec, bool grad) {
+    Shape s{256, 8, 1, 1};
     if (nvec <= 64 * 8) {
         s.nt = 64;
         s.nv = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
@@ -294,6 +277,9 @@ inline Shape distill_shape(int64_t n, int64_t v, int vec, bool grad) {
     s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv);
     return s;
 }
+inline int64_t distill_scratch(const Shape& s, int64_t n, int64_t k) {
+    return s.parts == 1 ? 0 : n * (16 + 8 * (int64_t)s.parts + 8 * k);
+}
 
 }  // namespace logits
 }  // namespace ddm
@@ -303,8 +289,10 @@ using namespace ddm::logits;
 
 extern "C" int64_t ddm_topk_distill_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t k, int32_t grad) {
     if (n <= 0 || v < 1 || v > kMaxColumns || k < 0 || k > kMaxTop) return 0;
-    const Shape s = distill_shape(n, v, dtype == DDM_F32 ? 4 : 8, grad != 0);
-    return s.parts == 1 ? 0 : n * (16 + 8 * (int64_t)s.parts + 8 * (int64_t)k);
+    const int vec = dtype == DDM_F32 ? 4 : 8;            // whether rows start aligned or not
+    const int64_t a = distill_scratch(distill_shape(n, ceil_div(v, vec), grad != 0), n, k);
+    const int64_t b = distill_scratch(distill_shape(n, ceil_div(v + vec - 1, vec), grad != 0), n, k);
+    return a > b ? a : b;
 }
 
 extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld, const void* index,
@@ -321,7 +309,8 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
         return DDM_E_ARG;
     }
     if (n == 0) return 0;
-    const Shape s = distill_shape(n, v, dtype == DDM_F32 ? 4 : 8, grad != nullptr);
+    const int size = dtype == DDM_F32 ? 4 : 2;
+    const Shape s = distill_shape(n, vectors_of(logits, ld * size, v, 16 / size), grad != nullptr);
     if (!logits || !loss || (k && (!index || !logprob)) || (grad && grad_ld < v) || (s.parts > 1 && !scratch)) {
         set_error("ddm_topk_distill: invalid argument (null pointer or gradient stride)");
         return DDM_E_ARG;

@@ -88,6 +88,12 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], f16_t) { return pack_
 // which those outside [0, v) are no entries.  Rows of an odd length start at any entry, so
 // `head` differs from row to row; only vectors that lie wholly inside are loaded as one,
 // the two at the ends entry by entry, and nothing outside the row is touched.
+// How many vectors the longest row of a matrix takes: one more if rows need not start aligned.
+inline int64_t vectors_of(const void* base, int64_t ld_bytes, int64_t v, int vec) {
+    const bool aligned = ((uintptr_t)base & 15) == 0 && ld_bytes % 16 == 0;
+    return ceil_div(v + (aligned ? 0 : vec - 1), vec);
+}
+
 template <typename T>
 struct Row {
     const char* base;    // address of column 0
@@ -163,6 +169,67 @@ struct Part {
 };
 __device__ __forceinline__ Part no_part() { return Part{-FLT_MAX, 0.0f, 0.0f}; }
 
+// A lane's own running sums, an entry in four operations and the exponential.  d is one fused
+// product, x log2(e) / T - scaled, with scaled = m log2(e) / T as float32 has it; what scaled lost in
+// rounding (`lost`) is given back at the end (part_of), exactly.  That needs scaled to be known to
+// a small part of one, so where it is over kWide (logits in the millions; rows masked by the type's
+// lowest value and little else) d is (x - m) log2(e) / T instead, for the waves that have such lanes.
+constexpr float kWide = 1048576.0f;
+struct Lane {
+    float m, scaled, wide;      // wide: entries from here on need the other form; +inf: none do
+    float s, u;
+};
+__device__ __forceinline__ Lane no_lane() { return Lane{-FLT_MAX, -3e38f, INFINITY, 0.0f, 0.0f}; }
+__device__ __forceinline__ float lost(const Lane& l, float c) {
+    return fabsf(l.scaled) > kWide ? 0.0f : -fmaf(l.m, c, -l.scaled);                       // scaled - m c
+}
+template <bool ENTROPY, int N>
+__device__ __forceinline__ void add_vector(Lane& l, const float (&f)[N], float most, float c) {
+    if (__any(most > l.m || (most == l.m && l.s == 0.0f))) {
+        Lane to = l;
+        to.m = fmaxf(l.m, most);
+        to.scaled = fminf(fmaxf(to.m * c, -3e38f), 3e38f);
+        float d = l.scaled - to.scaled;
+        if (__any(fabsf(l.scaled) > kWide || fabsf(to.scaled) > kWide)) {
+            d = (l.m - to.m) * c + (lost(l, c) - lost(to, c));
+            to.wide = fabsf(to.scaled) > kWide && (most >= -FLT_MAX || l.m > -FLT_MAX) ? -FLT_MAX : INFINITY;
+        }
+        d = fmaxf(d, kDead);
+        const float r = __builtin_amdgcn_exp2f(d);
+        if (ENTROPY) to.u = r * fmaf(l.s, d, l.u);
+        to.s = l.s * r;
+        l = to;
+    }
+    if (__any(most >= l.wide)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float d = l.wide < 0.0f ? (f[e] - l.m) * c : fmaf(f[e], c, -l.scaled);
+            const float w = __builtin_amdgcn_exp2f(d);
+            l.s += w;
+            if (ENTROPY) l.u = fmaf(w, fmaxf(d, kDead), l.u);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float d = fmaf(f[e], c, -l.scaled);
+        const float w = __builtin_amdgcn_exp2f(d);
+        l.s += w;
+        if (ENTROPY) l.u = fmaf(w, fmaxf(d, kDead), l.u);
+    }
+}
+__device__ __forceinline__ Part part_of(const Lane& l, float c) {
+    const float d = lost(l, c), r = __builtin_amdgcn_exp2f(d);
+    return Part{l.m, l.s * r, fmaf(d, l.s, l.u) * r};
+}
+template <int N>
+__device__ __forceinline__ float largest(const float (&f)[N]) {
+    float m = f[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) m = fmaxf(m, f[e]);
+    return m;
+}
+
 __device__ __forceinline__ void rebase(Part& a, float m, float c) {
     const float d = fmaxf((a.m - m) * c, kDead), r = __builtin_amdgcn_exp2f(d);
     a.u = r * fmaf(a.s, d, a.u);
@@ -185,6 +252,18 @@ __device__ __forceinline__ Part wave_merge(Part a, float c) {
         a = merge(a, b, c);
     }
     return a;
+}
+
+// ... and of a workgroup, in every lane.
+template <int NT>
+__device__ __forceinline__ Part block_merge(Part p, float c, Part* sh) {
+    constexpr int W = NT / 64;
+    p = wave_merge(p, c);
+    if (W == 1) return p;
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = p;
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    return wave_merge(lane < W ? sh[lane] : no_part(), c);
 }
 
 // float32 as an unsigned integer of the same order (-0 as +0); -inf is kKeyNegInf.
@@ -210,9 +289,8 @@ constexpr int kMaxTop = 64;              // alternatives of a row: one a lane
 constexpr int kMaxParts = 64;            // parts of a row, as well
 constexpr int64_t kMaxColumns = 1 << 19;
 
-// Lanes a workgroup, vectors a lane, workgroups a row.
 struct Shape {
-    int nt, nv, parts;
+    int nt, nv, turns, parts;    // a workgroup's part: turns times nv vectors a lane
 };
 template <typename F>
 int with_type(int32_t dtype, F f) {

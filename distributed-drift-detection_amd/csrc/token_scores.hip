@@ -24,7 +24,7 @@ struct ScoreArgs {
     const void* target;
     int target_wide;
     float temperature;
-    int top, parts;
+    int top, parts, turns;
     float *logprob, *entropy, *stats, *top_logprob;
     int32_t *rank, *top_index;
     uint8_t* err;
@@ -33,28 +33,50 @@ struct ScoreArgs {
 };
 
 // ---- the k largest of a workgroup's entries ----------------------------------------------------
-// A lane's largest entry is a lower bound with a witness of its own, so the k-th largest of a
-// wave's 64 lane maxima bounds the k-th largest entry from below; the best of the waves'
-// bounds leaves little more than k candidates, which go to LDS and are ordered by counting.
-// More candidates than the list holds (rows of equal values) are cut exactly by bisection.
+// A lane's largest entry is a lower bound with a witness of its own, so the k-th largest of the
+// lanes' bounds the k-th largest entry from below (tau).  Lanes whose largest reaches tau (little
+// more than k of them) have their entries read again, those that reach tau go to LDS and are
+// ordered by counting.  More of them than the list holds (rows of equal values) are cut exactly
+// by bisection, over entries read again each time: slow, but seldom, and bounded.
 struct SelectLds {
     uint64_t list[kListCap];
-    uint32_t tau[16], n, sum[16];
+    uint32_t keys[256], hits[kListCap];
+    uint32_t tau, n, nhits, sum[4];
 };
 
-// The k-th largest of the wave's keys (1 if fewer than k are above kKeyNegInf): bits from the
-// top, one ballot each; once exactly k remain, the prefix itself will do.
-__device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
-    uint32_t prefix = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t t = prefix | (1u << bit);
-        const int c = __popcll(__ballot(key >= t));
+// One wave: the k-th largest of NT keys in LDS (kKeyNegInf + 1 if fewer than k are above
+// kKeyNegInf).  Bits from the first one in which they differ, a ballot each; once exactly k
+// remain, the prefix itself will do.
+template <int NT>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* keys, int k) {
+    constexpr int N = NT / 64;
+    uint32_t key[N], all = 0xffffffffu, some = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        key[i] = keys[(threadIdx.x & 63) + 64 * i];
+        all &= key[i];
+        some |= key[i];
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        all &= __shfl_xor(all, d);
+        some |= __shfl_xor(some, d);
+    }
+    const uint32_t differ = __builtin_amdgcn_readfirstlane(all ^ some);
+    if (k > NT) return kKeyNegInf + 1;
+    uint32_t prefix = __builtin_amdgcn_readfirstlane(all);
+    if (differ) prefix &= ~((2u << (31 - __builtin_clz(differ))) - 1u);
+    for (uint32_t bit = differ ? 1u << (31 - __builtin_clz(differ)) : 0u; bit; bit >>= 1) {
+        const uint32_t t = prefix | bit;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(key[i] >= t));
         if (c >= k) {
             prefix = t;
             if (c == k) break;
         }
     }
-    return prefix > kKeyNegInf ? prefix : kKeyNegInf + 1;
+    return max(prefix, kKeyNegInf + 1);
 }
 
 template <int NT>
@@ -71,30 +93,52 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v, SelectLds& l) {
     return t;
 }
 
-// each(fn): fn(key, column) for every entry of the lane; out(rank, packed) for rank 0..k-1.
-template <int NT, class Each, class Out>
-__device__ __forceinline__ void select_top(SelectLds& l, uint32_t lane_max, int k, Each each, Out out) {
-    uint32_t tau = wave_kth(lane_max, k);
+__device__ __forceinline__ void keep(SelectLds& l, uint32_t key, uint32_t col) {
+    const uint32_t at = atomicAdd(&l.n, 1u);
+    if (at < (uint32_t)kListCap) l.list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
+}
+
+// best: the lane's largest key.  hits(tau, add): add(h) for what of the lane's reaches tau, a
+// number under 2^32 each; entries(h): how many entries one has, entry(h, i, fn): fn(key, column) of
+// the i-th, where there is one; each(fn): fn(key, column) for every entry of the lane.  out(rank,
+// packed) for rank 0..k-1.
+template <int NT, class Hits, class Entry, class Each, class Out>
+__device__ __forceinline__ void select_top(SelectLds& l, uint32_t best, int k, int entries, Hits hits, Entry entry,
+                                           Each each, Out out) {
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) l.tau[threadIdx.x >> 6] = tau;
-    if (threadIdx.x == 0) l.n = 0;
+    l.keys[threadIdx.x] = best;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) tau = max(tau, l.tau[w]);
-    if (lane_max >= tau)
-        each(tau, [&](uint32_t key, uint32_t col) {
-            const uint32_t at = atomicAdd(&l.n, 1u);
-            if (at < (uint32_t)kListCap) l.list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
+    if (threadIdx.x < 64) {
+        const uint32_t t = kth_largest<NT>(l.keys, k);
+        if (threadIdx.x == 0) {
+            l.tau = t;
+            l.n = 0;
+            l.nhits = 0;
+        }
+    }
+    __syncthreads();
+    const uint32_t tau = l.tau;
+    if (best >= tau)
+        hits(tau, [&](uint32_t h) {
+            const uint32_t at = atomicAdd(&l.nhits, 1u);
+            if (at < (uint32_t)kListCap) l.hits[at] = h;
         });
     __syncthreads();
+    const uint32_t nhits = l.nhits;
+    if (nhits <= (uint32_t)kListCap)
+        for (uint32_t i = threadIdx.x; i < nhits * (uint32_t)entries; i += NT)
+            entry(l.hits[i / (uint32_t)entries], (int)(i % (uint32_t)entries), [&](uint32_t key, uint32_t col) {
+                if (key >= tau) keep(l, key, col);
+            });
+    __syncthreads();
     uint32_t n = l.n;
-    if (n > (uint32_t)kListCap) {
+    if (n > (uint32_t)kListCap || nhits > (uint32_t)kListCap) {
         // the k-th value exactly (32 halvings), then how far its ties reach (32 more)
         uint32_t lo = tau, hi = 0xffffffffu;            // count(>= lo) >= k, and > hi holds none
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             uint32_t c = 0;
-            each(mid, [&](uint32_t, uint32_t) { ++c; });
+            each([&](uint32_t key, uint32_t) { c += key >= mid; });
             if (block_sum<NT>(c, l) >= (uint32_t)k)
                 lo = mid;
             else
@@ -102,13 +146,13 @@ __device__ __forceinline__ void select_top(SelectLds& l, uint32_t lane_max, int 
         }
         const uint32_t kth = lo;
         uint32_t more = 0;
-        each(kth, [&](uint32_t key, uint32_t) { more += key > kth; });
+        each([&](uint32_t key, uint32_t) { more += key > kth; });
         const uint32_t ties = (uint32_t)k - block_sum<NT>(more, l);
         uint32_t a = 0, b = 0xffffffffu;                // the lowest column with `ties` ties up to it
         while (a < b) {
             const uint32_t mid = a + (b - a) / 2;
             uint32_t c = 0;
-            each(kth, [&](uint32_t key, uint32_t col) { c += key == kth && col <= mid; });
+            each([&](uint32_t key, uint32_t col) { c += key == kth && col <= mid; });
             if (block_sum<NT>(c, l) >= ties)
                 b = mid;
             else
@@ -117,11 +161,8 @@ __device__ __forceinline__ void select_top(SelectLds& l, uint32_t lane_max, int 
         __syncthreads();
         if (threadIdx.x == 0) l.n = 0;
         __syncthreads();
-        each(kth, [&](uint32_t key, uint32_t col) {
-            if (key > kth || col <= a) {
-                const uint32_t at = atomicAdd(&l.n, 1u);
-                if (at < (uint32_t)kListCap) l.list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
-            }
+        each([&](uint32_t key, uint32_t col) {
+            if (key > kth || (key == kth && col <= a)) keep(l, key, col);
         });
         __syncthreads();
         n = min(l.n, (uint32_t)kListCap);
@@ -191,74 +232,61 @@ __device__ __forceinline__ void write_top(const ScoreArgs& a, int64_t r, const R
 // ---- a part of a row ---------------------------------------------------------------------------
 template <typename T, int NT, int NV, bool TOP>
 __global__ __launch_bounds__(NT) void k_score_parts(ScoreArgs a) {
-    constexpr int W = NT / 64;
     __shared__ SelectLds sel;
-    __shared__ Part sh_part[W];
-    __shared__ uint32_t sh_ahead[W];
+    __shared__ Part sh_part[NT / 64];
+    __shared__ uint32_t sh_ahead[NT / 64];
+    extern __shared__ uint32_t turn_best[];              // [turns][NT] the lanes' largest of each turn
     const int64_t r = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x % a.parts);
     const Row<T> row(a.x + r * a.ld_bytes, a.v);
-    const int j0 = part * NT * NV;
-    uint4 raw[NV];
-    load_part<T, NT, NV>(row, j0, raw);
+    const int turns = a.turns, j0 = part * NT * NV * turns;
 
     const float c = kLog2e / a.temperature;
     const int64_t t = target_at(a.target, a.target_wide, r);
     const bool counts = t >= 0 && t < a.v;
     const int t32 = counts ? (int)t : -1;
-    const float xt = counts ? row.at((int)t) : 0.0f;
+    const float xt = counts ? row.at(t32) : 0.0f;
     // entries before the target's column are ahead of it at equal value; a masked target has
     // every column before it ahead (added with the row) and the alive ones after it
     const float thr_after = counts ? xt : INFINITY;
     const float thr_before = counts && xt > -INFINITY ? below(xt) : INFINITY;
 
-    Part p = no_part();
-    float best[NV];
+    Lane sums = no_lane();
+    float best = -INFINITY;
     uint32_t ahead = 0;
+    for (int turn = 0; turn < turns; ++turn) {
+        const int jt = j0 + turn * NT * NV;
+        uint4 raw[NV];
+        load_part<T, NT, NV>(row, jt, raw);
+        float turn_most = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float f[T::kVec];
-        unpack(raw[i], f, T());
-        float m = f[0];
+        for (int i = 0; i < NV; ++i) {
+            float f[T::kVec];
+            unpack(raw[i], f, T());
+            const float most = largest(f);
+            turn_most = fmaxf(turn_most, most);
+            add_vector<true>(sums, f, most, c);
+            const float thr =
+                row.col(jt + i * NT + (int)threadIdx.x) + (T::kVec - 1) < t32 ? thr_before : thr_after;
+            if (__any(most > thr)) {
 #pragma unroll
-        for (int e = 1; e < T::kVec; ++e) m = fmaxf(m, f[e]);
-        best[i] = m;
-        if (__any(m > p.m)) rebase(p, fmaxf(p.m, m), c);
-        const float thr = row.col(j0 + i * NT + (int)threadIdx.x) + (T::kVec - 1) < t32 ? thr_before : thr_after;
-#pragma unroll
-        for (int e = 0; e < T::kVec; ++e) {
-            const float d = (f[e] - p.m) * c;
-            const float w = __builtin_amdgcn_exp2f(d);
-            p.s += w;
-            p.u = fmaf(w, fmaxf(d, kDead), p.u);
-            ahead += (uint32_t)__popcll(__ballot(f[e] > thr));
+                for (int e = 0; e < T::kVec; ++e) ahead += (uint32_t)__popcll(__ballot(f[e] > thr));
+            }
         }
+        best = fmaxf(best, turn_most);
+        if (TOP) turn_best[turn * NT + threadIdx.x] = key_of(turn_most);
     }
-    float lane_best = best[0];
-#pragma unroll
-    for (int i = 1; i < NV; ++i) lane_best = fmaxf(lane_best, best[i]);
-    p = wave_merge(p, c);
-    if (W > 1) {
-        if ((threadIdx.x & 63) == 0) {
-            sh_part[threadIdx.x >> 6] = p;
-            sh_ahead[threadIdx.x >> 6] = ahead;
-        }
-        __syncthreads();
-        p = sh_part[0];
-        ahead = sh_ahead[0];
-#pragma unroll
-        for (int w = 1; w < W; ++w) {
-            p = merge(p, sh_part[w], c);
-            ahead += sh_ahead[w];
-        }
+    if (threadIdx.x == 0 && counts) {                    // the entries before it in its own vector
+        const int jt = row.vector_of(t32);
+        if (jt >= j0 && jt < j0 + NT * NV * turns)
+            for (int i = max(row.col(jt), 0); i < t32; ++i)
+                ahead += xt > -INFINITY ? (uint32_t)(row.at(i) == xt) : -(uint32_t)(row.at(i) > xt);
     }
+    if ((threadIdx.x & 63) == 0) sh_ahead[threadIdx.x >> 6] = ahead;
+    const Part p = block_merge<NT>(part_of(sums, c), c, sh_part);
     if (threadIdx.x == 0) {
-        if (counts) {                                  // the entries before it in its own vector
-            const int jt = row.vector_of(t32);
-            if (jt >= j0 && jt < j0 + NT * NV)
-                for (int i = max(row.col(jt), 0); i < t32; ++i)
-                    ahead += xt > -INFINITY ? (uint32_t)(row.at(i) == xt) : -(uint32_t)(row.at(i) > xt);
-        }
+#pragma unroll
+        for (int w = 1; w < NT / 64; ++w) ahead += sh_ahead[w];
         if (a.parts == 1)
             write_row<T>(a, r, p, ahead);
         else
@@ -266,21 +294,26 @@ __global__ __launch_bounds__(NT) void k_score_parts(ScoreArgs a) {
     }
     if (!TOP) return;
     const RowLog g = row_log(p);
+    // a hit is a lane's turn; its entries are read again, as single ones
+    auto column = [&](uint32_t turn, uint32_t lane, int i) {
+        return row.col(j0 + (int)(turn * NT * NV + lane) + i / T::kVec * NT) + i % T::kVec;
+    };
     select_top<NT>(
-        sel, key_of(lane_best), a.top,
-        [&](uint32_t tau, auto fn) {
-            const float at_least = of_key(tau);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (best[i] >= at_least) {
-                    float f[T::kVec];
-                    unpack(again(raw[i]), f, T());
-                    const int c0 = row.col(j0 + i * NT + (int)threadIdx.x);
-#pragma unroll
-                    for (int e = 0; e < T::kVec; ++e)
-                        if (f[e] >= at_least) fn(key_of(f[e]), (uint32_t)(c0 + e));
+        sel, key_of(best), a.top, NV * T::kVec,
+        [&](uint32_t tau, auto add) {
+            for (int turn = 0; turn < turns; ++turn)
+                if (turn_best[turn * NT + threadIdx.x] >= tau) add((uint32_t)turn << 8 | threadIdx.x);
+        },
+        [&](uint32_t h, int i, auto fn) {
+            const int col = column(h >> 8, h & 255u, i);
+            if (col >= 0 && col < row.v) fn(key_of(row.at(col)), (uint32_t)col);
+        },
+        [&](auto fn) {
+            for (int turn = 0; turn < turns; ++turn)
+                for (int i = 0; i < NV * T::kVec; ++i) {
+                    const int col = column(turn, threadIdx.x, i);
+                    if (col >= 0 && col < row.v) fn(key_of(row.at(col)), (uint32_t)col);
                 }
-            }
         },
         [&](int k, uint64_t packed) {
             if (a.parts == 1)
@@ -291,9 +324,8 @@ __global__ __launch_bounds__(NT) void k_score_parts(ScoreArgs a) {
 }
 
 // ---- the parts of a row joined -------------------------------------------------------------------
-template <typename T, bool TOP>
-__global__ __launch_bounds__(TOP ? 256 : 64) void k_score_join(ScoreArgs a) {
-    constexpr int NT = TOP ? 256 : 64, NC = kMaxParts * kMaxTop / NT;
+template <typename T, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void k_score_join(ScoreArgs a) {
     __shared__ SelectLds sel;
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x & 63;
@@ -313,21 +345,18 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void k_score_join(ScoreArgs a) {
     const RowLog g = row_log(p);
     const int n = a.parts * a.top;
     const uint64_t* from = a.part_top + r * n;
-    uint64_t cand[NC];
     uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int at = i * NT + (int)threadIdx.x;
-        cand[i] = at < n ? from[at] : 0;
-        best = max(best, (uint32_t)(cand[i] >> 32));
-    }
+    for (int i = threadIdx.x; i < n; i += NT) best = max(best, (uint32_t)(from[i] >> 32));
+    auto each = [&](auto fn) {
+        for (int i = threadIdx.x; i < n; i += NT) fn((uint32_t)(from[i] >> 32), ~(uint32_t)from[i]);
+    };
     select_top<NT>(
-        sel, best, a.top,
-        [&](uint32_t tau, auto fn) {
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-                if ((uint32_t)(cand[i] >> 32) >= tau) fn((uint32_t)(cand[i] >> 32), ~(uint32_t)cand[i]);
+        sel, best, a.top, 1,
+        [&](uint32_t tau, auto add) {
+            for (int i = threadIdx.x; i < n; i += NT)
+                if ((uint32_t)(from[i] >> 32) >= tau) add((uint32_t)i);
         },
+        [&](uint32_t h, int, auto fn) { fn((uint32_t)(from[h] >> 32), ~(uint32_t)from[h]); }, each,
         [&](int k, uint64_t packed) { write_top(a, r, g, k, packed); });
 }
 
@@ -409,21 +438,22 @@ __global__ __launch_bounds__(NT) void k_score_grad(GradArgs a) {
 
 // ---- launch shapes ---------------------------------------------------------------------------------
 // One wave a row while the row fits its registers (512 vectors of 16 bytes); longer rows in
-// parts of 256 lanes, 8 vectors each, or fewer while there are not workgroups enough to fill
-// 256 CUs several times over.
-inline Shape shape_of(int64_t n, int64_t v, int vec) {
-    const int64_t nvec = ceil_div(v + vec - 1, vec);     // whatever the rows' alignment
-    Shape s;
+// parts of 256 lanes, 8 vectors a lane and turn, with as many turns (a selection a part) or as
+// few vectors as leave workgroups enough to fill 256 CUs several times over.
+inline Shape shape_of(int64_t n, int64_t nvec, bool turns) {
+    Shape s{256, 8, 1, 1};
     if (nvec <= 64 * 8) {
         s.nt = 64;
         s.nv = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
     } else {
-        s.nt = 256;
-        s.nv = 8;
         while (s.nv > 1 && n * ceil_div(nvec, 256 * s.nv) < 1024 && ceil_div(nvec, 128 * s.nv) <= kMaxParts) s.nv /= 2;
+        while (turns && s.turns < 4 && n * ceil_div(nvec, 256 * s.nv * s.turns * 2) >= 4096) s.turns *= 2;
     }
-    s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv);
+    s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv * s.turns);
     return s;
+}
+inline int64_t score_scratch(const Shape& s, int64_t n, int64_t top) {
+    return s.parts == 1 ? 0 : n * s.parts * (16 + 8 * top);
 }
 
 }  // namespace logits
@@ -434,8 +464,10 @@ using namespace ddm::logits;
 
 extern "C" int64_t ddm_token_scores_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t top) {
     if (n <= 0 || v < 1 || v > kMaxColumns || top < 0 || top > kMaxTop) return 0;
-    const Shape s = shape_of(n, v, dtype == DDM_F32 ? 4 : 8);
-    return s.parts == 1 ? 0 : n * s.parts * (16 + 8 * (int64_t)top);
+    const int vec = dtype == DDM_F32 ? 4 : 8;            // whether rows start aligned or not
+    const int64_t a = score_scratch(shape_of(n, ceil_div(v, vec), true), n, top);
+    const int64_t b = score_scratch(shape_of(n, ceil_div(v + vec - 1, vec), true), n, top);
+    return a > b ? a : b;
 }
 
 extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld,
@@ -445,7 +477,8 @@ extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, in
                                 ddm_event_t ev_begin, ddm_event_t ev_end) {
     if (int rc = check_rows("ddm_token_scores", dtype, n, v, ld, target_bytes, temperature, top)) return rc;
     if (n == 0) return 0;
-    const Shape s = shape_of(n, v, dtype == DDM_F32 ? 4 : 8);
+    const int size = dtype == DDM_F32 ? 4 : 2;
+    const Shape s = shape_of(n, vectors_of(logits, ld * size, v, 16 / size), true);
     if (!logits || !target || !logprob || !entropy || !stats || !rank || !err || (top && (!top_logprob || !top_index)) ||
         (s.parts > 1 && !scratch)) {
         set_error("ddm_token_scores: invalid argument (null pointer)");
@@ -456,20 +489,22 @@ extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, in
         return with_type(dtype, [&](auto type) {
             using T = decltype(type);
             ScoreArgs a{(const char*)logits, n, v, ld * T::kSize, target, target_bytes == 8, temperature, top, s.parts,
-                        logprob, entropy, stats, top_logprob, rank, top_index, err, (float4*)scratch,
+                        s.turns, logprob, entropy, stats, top_logprob, rank, top_index, err, (float4*)scratch,
                         (uint64_t*)((char*)scratch + n * s.parts * 16)};
             with_part_shape(s, [&](auto nt, auto nv) {
                 if (top)
-                    k_score_parts<T, nt(), nv(), true><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
+                    k_score_parts<T, nt(), nv(), true><<<dim3((unsigned)(n * s.parts)), nt(), nt() * s.turns * 4, st>>>(a);
                 else
                     k_score_parts<T, nt(), nv(), false><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
             });
             if (int rc = launch_status("ddm_token_scores")) return rc;
             if (s.parts > 1) {
-                if (top)
-                    k_score_join<T, true><<<dim3((unsigned)n), 256, 0, st>>>(a);
+                if (!top)
+                    k_score_join<T, 64, false><<<dim3((unsigned)n), 64, 0, st>>>(a);
+                else if (s.parts * top <= 512)                 // 8 a lane: a wave is enough
+                    k_score_join<T, 64, true><<<dim3((unsigned)n), 64, 0, st>>>(a);
                 else
-                    k_score_join<T, false><<<dim3((unsigned)n), 64, 0, st>>>(a);
+                    k_score_join<T, 256, true><<<dim3((unsigned)n), 256, 0, st>>>(a);
             }
             return launch_status("ddm_token_scores");
         });
@@ -487,7 +522,8 @@ extern "C" int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t 
         set_error("ddm_token_scores_grad: invalid argument (null pointer or output stride)");
         return DDM_E_ARG;
     }
-    const Shape s = shape_of(n, v, dtype == DDM_F32 ? 4 : 8);
+    const int size = dtype == DDM_F32 ? 4 : 2;
+    const Shape s = shape_of(n, vectors_of(logits, ld * size, v, 16 / size), false);
     const hipStream_t st = as_hip(stream);
     return timed(ev_begin, ev_end, st, [&] {
         return with_type(dtype, [&](auto type) {
