@@ -12,12 +12,15 @@
 // the part in LDS, and p_i / p_r is the softmax over the others, so nothing overflows where
 // p_r does not fit float32 either.
 //
-// Bound by reading the logits once and writing the gradient once.  A row that fits one
-// workgroup's registers (1024 lanes of 16 vectors: 131072 16-bit entries) is read once, summed
-// while it arrives, and written from the registers; longer rows, and rows too few to fill the
-// chip with a workgroup each, are cut into parts, summed, finished by a wave a row and written
-// by a second reading.
+// Bound by reading the logits once and writing the gradient once.  A part of a row (256 lanes of 8
+// vectors) stays in a workgroup's registers while the row's parts tell each other their sums, and
+// is written from there: every logit is read once, and with 6 workgroups on a CU the others load or
+// store while one waits.  The row's first part finishes it: it alone looks up the student's logits at
+// the teacher's columns (64 lines a row) and writes the gradient there, so the other parts leave
+// those columns out.  (A whole row in the registers of 1024 lanes leaves one workgroup a CU and
+// nothing to do while it sums; reading twice costs half again the traffic.)
 #include "logits.h"
+#include "words.h"
 
 namespace ddm {
 namespace logits {
@@ -33,10 +36,9 @@ struct DistillArgs {
     float temperature;
     float* loss;
     char* out;                 // NULL: the loss alone
-    float2* part_sum;          // [n][parts] m, s of what is not kept (renorm: of everything)
-    float4* coef;              // [n] the bulk's m, log2 s and factor
-    int32_t* kept;             // [n][k] column, or -1
-    float* kept_grad;          // [n][k]
+    uint32_t *tickets, queues; // one part a row: NULL
+    uint64_t* words;           // [n][parts + 2]: m, s of a part's columns that are not kept (renorm: of
+                               // all); then the row's Bulk
 };
 
 // The teacher's alternatives of a row, one a lane of a wave.
@@ -46,16 +48,17 @@ struct Kept {
 };
 
 template <typename T>
-__device__ __forceinline__ Kept load_kept(const DistillArgs& a, int64_t r, const Row<T>& row) {
+__device__ __forceinline__ Kept load_kept(const DistillArgs& a, int64_t r, int col, const Row<T>& row) {
     const int lane = threadIdx.x & 63;
-    Kept k{-1, -INFINITY, -INFINITY};
-    if (lane < a.k) {
-        const int64_t c = target_at(a.index, a.index_wide, r * a.k + lane);
-        k.col = c >= 0 && c < a.v ? (int)c : -1;
-        k.l = a.logprob[r * a.k + lane];
+    Kept k{col, -INFINITY, -INFINITY};
+    if (lane < a.k) k.l = a.logprob[r * a.k + lane];
+    uint64_t same = __ballot(k.col >= 0);                // lanes of the same column, a bit of it at a time
+    for (int bit = 0; bit < 19; ++bit) {
+        const bool one = k.col >> bit & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
     }
-    for (int j = 0; j + 1 < a.k; ++j)                    // the first of equal columns counts
-        if (lane > j && k.col == __builtin_amdgcn_readlane(k.col, j)) k.col = -1;
+    if (k.col >= 0 && (same & ((1ull << lane) - 1ull))) k.col = -1;      // the first of equal ones counts
     if (k.col >= 0)
         k.x = row.at(k.col);
     else
@@ -155,131 +158,120 @@ __device__ __forceinline__ Part sum_part(const uint4 (&raw)[NV], float c, bool r
     return part_of(l, c);
 }
 
-template <typename T>
-__device__ __forceinline__ void write_vector(const Row<T>& row, char* out, int j, const uint4& raw, float c,
-                                             const Bulk& b) {
-    float f[T::kVec];
-    unpack(raw, f, T());
+// The gradient of a column that is not kept: 2^(x c - shift) * factor, one fused product an entry.
+// What shift = m c + log2 s loses in rounding is in the factor; where it is too large for that (see
+// add_vector) the difference x - m comes first.
+struct Writer {
+    float m, log2_s, shift, factor;
+    bool wide;
+};
+__device__ __forceinline__ Writer writer_of(const Bulk& b, float c) {
+    Writer w{b.m, b.log2_s, fmaf(b.m, c, b.log2_s), b.factor, false};
+    w.wide = !(fabsf(w.shift) < kWide);
+    if (!w.wide) w.factor *= __builtin_amdgcn_exp2f(-(fmaf(b.m, c, -w.shift) + b.log2_s));
+    return w;
+}
+template <int N>
+__device__ __forceinline__ void gradient(float (&f)[N], float c, const Writer& w) {
+    if (w.wide || w.factor == 0.0f) {
 #pragma unroll
-    for (int e = 0; e < T::kVec; ++e)
-        f[e] = b.factor == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((f[e] - b.m) * c - b.log2_s) * b.factor;
-    row.store(out, j, f);
+        for (int e = 0; e < N; ++e)
+            f[e] = w.factor == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((f[e] - w.m) * c - w.log2_s) * w.factor;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = __builtin_amdgcn_exp2f(fmaf(f[e], c, -w.shift)) * w.factor;
+    }
 }
 
-// ---- a row in one workgroup's registers -------------------------------------------------------------
+__device__ __forceinline__ uint64_t wait_for(const uint64_t* p) {
+    uint64_t w = peek(p);
+    for (uint32_t spin = 0; w == kUnset && spin < kSpinLimit; ++spin) {
+        __builtin_amdgcn_s_sleep(1);
+        w = peek(p);
+    }
+    return w;                                            // unset: NaN
+}
+
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void k_distill_rows(DistillArgs a) {
+__global__ __launch_bounds__(NT) void k_distill(DistillArgs a) {
     __shared__ uint32_t bits[NT * NV / 4];
     __shared__ Part sh_part[NT / 64];
     __shared__ Bulk sh_bulk;
-    const int64_t r = blockIdx.x;
+    // a queue gives out the parts of every queues-th row, row by row: the parts of all but its last row
+    // run, so no more than queues * (parts - 1) workgroups ever wait for one that has not begun
+    Ticket at{0u, blockIdx.x};
+    if (a.tickets) at = take_ticket(a.tickets, a.queues);
+    const int64_t r = (int64_t)(at.number / (uint32_t)a.parts) * a.queues + at.queue;
+    const int part = (int)(at.number % (uint32_t)a.parts), j0 = part * NT * NV;
+    if (r >= a.n) return;
     const Row<T> row(a.x + r * a.ld_bytes, a.v);
     uint4 raw[NV];
-    load_part<T, NT, NV>(row, 0, raw);
+    load_part<T, NT, NV>(row, j0, raw);
     const float c = kLog2e / a.temperature;
+    int col = -1;
+    if ((int)threadIdx.x < a.k) {
+        const int64_t i = target_at(a.index, a.index_wide, r * a.k + threadIdx.x);
+        col = i >= 0 && i < a.v ? (int)i : -1;
+    }
+    mark_kept<NT, NV>(bits, col >= 0, col >= 0 ? row.vector_of(col) - j0 : -1, (col + row.head) % T::kVec);
     Kept k{-1, 0.0f, 0.0f};
-    if (threadIdx.x < 64) k = load_kept(a, r, row);
-    if (a.rest) mark_kept<NT, NV>(bits, k.col >= 0, row.vector_of(k.col), (k.col + row.head) % T::kVec);
-    const Part p = block_merge<NT>(sum_part<T, NT, NV>(raw, c, a.rest, bits), c, sh_part);
+    const bool finish = part == 0 && threadIdx.x < 64;
+    if (finish) k = load_kept(a, r, col, row);
+    Part p = block_merge<NT>(sum_part<T, NT, NV>(raw, c, a.rest, bits), c, sh_part);
+    uint64_t* words = a.words + r * (a.parts + 2);
+    if (a.tickets && threadIdx.x == 0) publish(words + part, word(p.m, p.s));
     float kept_grad = 0.0f;
-    if (threadIdx.x < 64) {
+    if (finish) {
+        if (a.tickets) {
+            p = no_part();
+            if ((int)threadIdx.x < a.parts) {
+                const uint64_t w = wait_for(words + threadIdx.x);
+                p.m = word_a(w);
+                p.s = word_b(w);
+            }
+            p = wave_merge(p, c);
+        }
         const Bulk b = finish_row<T>(a, r, k, p, kept_grad);
-        if (threadIdx.x == 0) sh_bulk = b;
+        if (threadIdx.x == 0) {
+            sh_bulk = b;
+            if (a.tickets && a.out) {
+                publish(words + a.parts, word(b.m, b.log2_s));
+                publish(words + a.parts + 1, word(b.factor, 0.0f));
+            }
+        }
     }
     if (!a.out) return;
+    if (part != 0 && threadIdx.x == 0) {
+        const uint64_t w = wait_for(words + a.parts), f = wait_for(words + a.parts + 1);
+        sh_bulk = Bulk{word_a(w), word_b(w), word_a(f)};
+    }
     __syncthreads();
-    const Bulk b = sh_bulk;
+    const Writer w = writer_of(sh_bulk, c);
     char* out = a.out + r * a.out_ld_bytes;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) write_vector(row, out, i * NT + (int)threadIdx.x, again(raw[i]), c, b);
-    __syncthreads();
-    if (threadIdx.x < 64 && k.col >= 0) T::store(out + k.col * T::kSize, kept_grad);
+    store_part<T, NT, NV>(
+        row, out, j0,
+        [&](int i, float (&f)[T::kVec]) {
+            unpack(again(raw[i]), f, T());
+            gradient(f, c, w);
+        },
+        [&](int i) { return (uint32_t)((const uint8_t*)bits)[i * NT + threadIdx.x]; });
+    if (finish && k.col >= 0) T::store(out + k.col * T::kSize, kept_grad);
 }
 
-// ---- rows in parts ------------------------------------------------------------------------------------
-template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void k_distill_parts(DistillArgs a) {
-    __shared__ uint32_t bits[NT * NV / 4];
-    __shared__ Part sh_part[NT / 64];
-    const int64_t r = blockIdx.x / a.parts;
-    const int part = (int)(blockIdx.x % a.parts), j0 = part * NT * NV;
-    const Row<T> row(a.x + r * a.ld_bytes, a.v);
-    uint4 raw[NV];
-    load_part<T, NT, NV>(row, j0, raw);
-    const float c = kLog2e / a.temperature;
-    if (a.rest) {                                       // repeats set the same bit twice
-        int64_t col = -1;
-        if (threadIdx.x < a.k) col = target_at(a.index, a.index_wide, r * a.k + threadIdx.x);
-        const bool in = col >= 0 && col < a.v;
-        mark_kept<NT, NV>(bits, in, in ? row.vector_of((int)col) - j0 : -1, in ? ((int)col + row.head) % T::kVec : 0);
-    }
-    const Part p = block_merge<NT>(sum_part<T, NT, NV>(raw, c, a.rest, bits), c, sh_part);
-    if (threadIdx.x == 0) a.part_sum[r * a.parts + part] = make_float2(p.m, p.s);
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void k_distill_join(DistillArgs a) {
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x;
-    const Row<T> row(a.x + r * a.ld_bytes, a.v);
-    const Kept k = load_kept(a, r, row);
-    Part p = no_part();
-    if (lane < a.parts) {
-        const float2 q = a.part_sum[r * a.parts + lane];
-        p.m = q.x;
-        p.s = q.y;
-    }
-    p = wave_merge(p, kLog2e / a.temperature);
-    float kept_grad;
-    const Bulk b = finish_row<T>(a, r, k, p, kept_grad);
-    if (!a.out) return;
-    if (lane == 0) a.coef[r] = make_float4(b.m, b.log2_s, b.factor, 0.0f);
-    if (lane < a.k) {
-        a.kept[r * a.k + lane] = k.col;
-        a.kept_grad[r * a.k + lane] = kept_grad;
-    }
-}
-
-template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs a) {
-    const int64_t r = blockIdx.x / a.parts;
-    const int part = (int)(blockIdx.x % a.parts), j0 = part * NT * NV;
-    const Row<T> row(a.x + r * a.ld_bytes, a.v);
-    uint4 raw[NV];
-    load_part<T, NT, NV>(row, j0, raw);
-    const float4 q = a.coef[r];
-    const Bulk b{q.x, q.y, q.z};
-    const float c = kLog2e / a.temperature;
-    char* out = a.out + r * a.out_ld_bytes;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) write_vector(row, out, j0 + i * NT + (int)threadIdx.x, raw[i], c, b);
-    __syncthreads();
-    if (threadIdx.x < a.k) {
-        const int col = a.kept[r * a.k + threadIdx.x];
-        const int j = col >= 0 ? row.vector_of(col) - j0 : -1;
-        if (j >= 0 && j < NT * NV) T::store(out + col * T::kSize, a.kept_grad[r * a.k + threadIdx.x]);
-    }
-}
-
-// A workgroup a row while it fits and there are rows enough to give every CU one or two, or
-// nothing is gained by cutting it; parts as for the scores otherwise.
-inline Shape distill_shape(int64_t n, int64_t nvec, bool grad) {
+// A wave a row while the row fits its registers; 256 lanes and 8 vectors beyond, or fewer vectors
+// while that leaves too few workgroups to fill 256 CUs.
+inline Shape distill_shape(int64_t n, int64_t nvec) {
     Shape s{256, 8, 1, 1};
     if (nvec <= 64 * 8) {
         s.nt = 64;
         s.nv = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
-    } else if (grad && n >= 256 && nvec <= 1024 * 16) {
-        s.nt = nvec <= 256 * 8 ? 256 : 1024;
-        s.nv = nvec <= 256 * 4 ? 4 : nvec <= 256 * 8 ? 8 : nvec <= 1024 * 4 ? 4 : nvec <= 1024 * 8 ? 8 : 16;
     } else {
         while (s.nv > 1 && n * ceil_div(nvec, 256 * s.nv) < 1024 && ceil_div(nvec, 128 * s.nv) <= kMaxParts) s.nv /= 2;
     }
     s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv);
     return s;
 }
-inline int64_t distill_scratch(const Shape& s, int64_t n, int64_t k) {
-    return s.parts == 1 ? 0 : n * (16 + 8 * (int64_t)s.parts + 8 * k);
-}
+inline int64_t distill_scratch(const Shape& s, int64_t n) { return s.parts == 1 ? 0 : kTicketBytes + 8 * n * (s.parts + 2); }
 
 }  // namespace logits
 }  // namespace ddm
@@ -287,11 +279,11 @@ inline int64_t distill_scratch(const Shape& s, int64_t n, int64_t k) {
 using namespace ddm;
 using namespace ddm::logits;
 
-extern "C" int64_t ddm_topk_distill_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t k, int32_t grad) {
-    if (n <= 0 || v < 1 || v > kMaxColumns || k < 0 || k > kMaxTop) return 0;
+extern "C" int64_t ddm_topk_distill_scratch_bytes(int64_t n, int64_t v, int32_t dtype) {
+    if (n <= 0 || v < 1 || v > kMaxColumns) return 0;
     const int vec = dtype == DDM_F32 ? 4 : 8;            // whether rows start aligned or not
-    const int64_t a = distill_scratch(distill_shape(n, ceil_div(v, vec), grad != 0), n, k);
-    const int64_t b = distill_scratch(distill_shape(n, ceil_div(v + vec - 1, vec), grad != 0), n, k);
+    const int64_t a = distill_scratch(distill_shape(n, ceil_div(v, vec)), n);
+    const int64_t b = distill_scratch(distill_shape(n, ceil_div(v + vec - 1, vec)), n);
     return a > b ? a : b;
 }
 
@@ -310,7 +302,7 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
     }
     if (n == 0) return 0;
     const int size = dtype == DDM_F32 ? 4 : 2;
-    const Shape s = distill_shape(n, vectors_of(logits, ld * size, v, 16 / size), grad != nullptr);
+    const Shape s = distill_shape(n, vectors_of(logits, ld * size, v, 16 / size));
     if (!logits || !loss || (k && (!index || !logprob)) || (grad && grad_ld < v) || (s.parts > 1 && !scratch)) {
         set_error("ddm_topk_distill: invalid argument (null pointer or gradient stride)");
         return DDM_E_ARG;
@@ -319,27 +311,18 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
     return timed(ev_begin, ev_end, st, [&] {
         return with_type(dtype, [&](auto type) {
             using T = decltype(type);
-            char* w = (char*)scratch;
             DistillArgs a{(const char*)logits, n, v, ld * T::kSize, grad_ld * T::kSize, index, index_bytes == 8, logprob,
-                          weight, k, tail == DDM_TAIL_REST, s.parts, temperature, loss, (char*)grad,
-                          (float2*)(w + n * 16), (float4*)w, (int32_t*)(w + n * (16 + 8 * (int64_t)s.parts)),
-                          (float*)(w + n * (16 + 8 * (int64_t)s.parts + 4 * (int64_t)k))};
-            if (s.parts == 1) {
-                with_row_shape(s, [&](auto nt, auto nv) { k_distill_rows<T, nt(), nv()><<<dim3((unsigned)n), nt(), 0, st>>>(a); });
-                return launch_status("ddm_topk_distill");
+                          weight, k, tail == DDM_TAIL_REST, s.parts, temperature, loss, (char*)grad, nullptr, 1, nullptr};
+            if (s.parts > 1) {
+                a.tickets = (uint32_t*)scratch;
+                while (a.queues < kQueues && a.queues * 2 * s.parts <= 128) a.queues *= 2;
+                a.words = (uint64_t*)((char*)scratch + kTicketBytes);
+                if (int rc = reset_words(a.tickets, a.words, n * (s.parts + 2), nullptr, nullptr, 0, st, "ddm_topk_distill"))
+                    return rc;
             }
-            const dim3 grid((unsigned)(n * s.parts));
-            auto each_part = [&](auto launch) {
-                if (s.nv == 1) launch(std::integral_constant<int, 1>());
-                if (s.nv == 2) launch(std::integral_constant<int, 2>());
-                if (s.nv == 4) launch(std::integral_constant<int, 4>());
-                if (s.nv == 8) launch(std::integral_constant<int, 8>());
-            };
-            each_part([&](auto nv) { k_distill_parts<T, 256, nv()><<<grid, 256, 0, st>>>(a); });
-            if (int rc = launch_status("ddm_topk_distill")) return rc;
-            k_distill_join<T><<<dim3((unsigned)n), 64, 0, st>>>(a);
-            if (int rc = launch_status("ddm_topk_distill")) return rc;
-            if (grad) each_part([&](auto nv) { k_distill_grad<T, 256, nv()><<<grid, 256, 0, st>>>(a); });
+            with_part_shape(s, [&](auto nt, auto nv) {
+                k_distill<T, nt(), nv()><<<dim3((unsigned)(ceil_div(n, a.queues) * a.queues * s.parts)), nt(), 0, st>>>(a);
+            });
             return launch_status("ddm_topk_distill");
         });
     });

@@ -26,14 +26,12 @@
 #include <initializer_list>
 #include <type_traits>
 
-#include "common.h"
+#include "words.h"
 
 namespace ddm {
 namespace gated {
 
 constexpr int NT = 512, W = NT / 64;
-constexpr uint64_t kUnset = ~0ull;
-constexpr uint32_t kSpinLimit = 1u << 22;      // a tile's predecessors run already: a guard, not a wait
 constexpr float kCut = -1.0f;                   // A of a step that forgets what was before it
 
 template <typename E_, int CODE>
@@ -85,7 +83,7 @@ struct Args {
     float* state_out;                     // state after, or gradient of the state before
     int cl_bits, ncb, group;             // lanes across channels (log2), channel blocks, tiles a group
     int64_t ntiles;
-    uint32_t* ticket;                     // NULL: one tile, no chain
+    uint32_t *tickets, queues;            // NULL: one tile, no chain
     uint64_t *agg, *inc;                  // [ntiles][dp], [groups][dp]
     int64_t dp;
     float* dl_part;                       // [rows][parts a row] or NULL: dl itself
@@ -157,14 +155,11 @@ struct Place {
     int block;             // of channels
 };
 __device__ __forceinline__ Place take(const Args& a) {
-    __shared__ uint32_t sh;
-    uint32_t t = blockIdx.x;
-    if (a.ticket) {
-        if (threadIdx.x == 0) sh = atomicAdd(a.ticket, 1u);
-        __syncthreads();
-        t = __builtin_amdgcn_readfirstlane(sh);      // the same in every lane, and known to be
-    }
-    return Place{(int64_t)(t / (uint32_t)a.ncb), (int)(t % (uint32_t)a.ncb)};
+    if (!a.tickets) return Place{(int64_t)(blockIdx.x / (uint32_t)a.ncb), (int)(blockIdx.x % (uint32_t)a.ncb)};
+    // a queue gives out all tiles of every queues-th channel block, tile by tile
+    const Ticket t = take_ticket(a.tickets, a.queues);
+    const uint32_t blocks = (uint32_t)a.ncb / a.queues;
+    return Place{(int64_t)(t.number / blocks), (int)(t.number % blocks * a.queues + t.queue)};
 }
 
 // Which rows of a tile begin and end a sequence: a bit a row, and the sequence's number where it is set.
@@ -224,19 +219,6 @@ struct ScanLds {
     float a[W][64 * VEC], b[W][64 * VEC];
 };
 
-__device__ __forceinline__ uint64_t pack(float a, float b) {
-    const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-    return w == kUnset ? w ^ 1u : w;               // two NaN of all ones: another NaN
-}
-__device__ __forceinline__ Step unpack(uint64_t w) {
-    return Step{__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
-}
-__device__ __forceinline__ void publish(uint64_t* p, uint64_t w) {
-    __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ uint64_t peek(const uint64_t* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 // The first `count` (at most N) words of a column, all asked for at once; unset ones, if the guard
 // ever ran out, are NaN.
 template <int N>
@@ -290,11 +272,11 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
 #pragma unroll
         for (int w = 0; w < W; ++w) all = after(all, Step{l.a[w][col], l.b[w][col]});
         float carry = 0.0f;
-        if (a.ticket) {
+        if (a.tickets) {
             const int64_t c = (int64_t)at.block * cols + col, g = at.tile / a.group;
             const int in_group = (int)(at.tile % a.group);
             const bool last = in_group == a.group - 1, more = at.tile + 1 < a.ntiles;
-            if (!last && more) publish(a.agg + at.tile * a.dp + c, pack(all.a, all.b));
+            if (!last && more) publish(a.agg + at.tile * a.dp + c, word(all.a, all.b));
             // the tiles before in the group first: they run beside this one; the group before is
             // what there may be a wait for
             Step sum{1.0f, 0.0f};
@@ -303,15 +285,15 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
                 await<8>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (j + i < in_group) sum = after(sum, unpack(w[i]));
+                    if (j + i < in_group) sum = after(sum, Step{word_a(w[i]), word_b(w[i])});
             }
             if (g > 0) {
                 uint64_t w[1];
                 await<1>(a.inc + (g - 1) * a.dp + c, 0, 1, w);
-                carry = unpack(w[0]).a;
+                carry = word_a(w[0]);
             }
             carry = apply(sum, carry);
-            if (last && more) publish(a.inc + g * a.dp + c, pack(apply(all, carry), 0.0f));
+            if (last && more) publish(a.inc + g * a.dp + c, word(apply(all, carry), 0.0f));
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -460,7 +442,7 @@ inline int check_tile(const char* who, const Shape& s, std::initializer_list<int
 
 inline int64_t scratch_bytes(const Shape& s, int64_t rows, int d) {
     const int64_t parts = s.dl_parts ? rows * (d / (s.vec * s.dl_width)) : 0;
-    return (s.words() ? 16 + 8 * s.words() : 0) + 4 * parts;
+    return (s.words() ? kTicketBytes + 8 * s.words() : 0) + 4 * parts;
 }
 
 // The chain's buffers and the copy of the states, with their launch where either is needed (gated.hip).

@@ -121,17 +121,6 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     }
 }
 
-// Before a scan: what the chain waits for is unset, and every sequence's state goes through
-// (those with rows write theirs afterwards).
-__global__ __launch_bounds__(256) void k_gated_begin(uint32_t* ticket, uint64_t* words, int64_t nwords,
-                                                     const float* from, float* to, int64_t nstate) {
-    const int64_t step = (int64_t)gridDim.x * 256;
-    const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i0 == 0 && ticket) *ticket = 0;
-    for (int64_t i = i0; i < nwords; i += step) words[i] = kUnset;
-    for (int64_t i = i0; i < nstate; i += step) to[i] = from ? from[i] : 0.0f;
-}
-
 // One row a sequence: elementwise, the state's row beside it.
 template <typename X, typename L, int VEC, bool OWN>
 __global__ __launch_bounds__(256) void k_gated_step(Args a) {
@@ -163,10 +152,11 @@ int begin(Args& a, const Shape& s, void* scratch, const float* from, float* to, 
     char* w = (char*)scratch;
     const int64_t words = s.words();
     if (words) {
-        a.ticket = (uint32_t*)w;
-        a.agg = (uint64_t*)(w + 16);
+        a.tickets = (uint32_t*)w;
+        a.queues = s.ncb % 8 == 0 ? 8 : s.ncb % 4 == 0 ? 4 : s.ncb % 2 == 0 ? 2 : 1;
+        a.agg = (uint64_t*)(w + kTicketBytes);
         a.inc = a.agg + s.ntiles * s.dp;
-        w += 16 + 8 * words;
+        w += kTicketBytes + 8 * words;
     }
     if (s.dl_parts) a.dl_part = (float*)w;
     a.cl_bits = s.cl_bits;
@@ -175,11 +165,8 @@ int begin(Args& a, const Shape& s, void* scratch, const float* from, float* to, 
     a.ntiles = s.ntiles;
     a.dp = s.dp;
     a.dl_width = s.dl_width;
-    const int64_t most = words > nstate ? words : nstate;
     if (!words && !a.off && s.ntiles) return 0;        // one tile, one sequence that has rows
-    const int64_t grid = ceil_div(most, 256 * 4) < 2048 ? ceil_div(most, 256 * 4) : 2048;
-    k_gated_begin<<<dim3((unsigned)(grid > 0 ? grid : 1)), 256, 0, st>>>(a.ticket, a.agg, words, from, to, nstate);
-    return launch_status("ddm_gated_scan");
+    return reset_words(a.tickets, a.agg, words, from, to, nstate, st, "ddm_gated_scan");
 }
 
 }  // namespace gated

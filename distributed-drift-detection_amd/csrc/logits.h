@@ -126,31 +126,54 @@ struct Row {
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    // The vector's entries into another row (gradients), as one where that is aligned alike.
-    __device__ __forceinline__ void store(char* out, int j, const float (&f)[T::kVec]) const {
+    // The vector's entries into another row (gradients), as one where that is aligned alike; but for
+    // those with a bit in `without`.
+    __device__ __forceinline__ void store(char* out, int j, const float (&f)[T::kVec], uint32_t without = 0) const {
         const int c0 = col(j);
         char* p = out + c0 * T::kSize;
-        if (whole(j) && ((uintptr_t)p & 15) == 0) {
+        if (whole(j) && ((uintptr_t)p & 15) == 0 && without == 0) {
             *(uint4*)p = pack(f, T());
             return;
         }
 #pragma unroll
         for (int e = 0; e < T::kVec; ++e)
-            if (c0 + e >= 0 && c0 + e < v) T::store(p + e * T::kSize, f[e]);
+            if (c0 + e >= 0 && c0 + e < v && !(without >> e & 1)) T::store(p + e * T::kSize, f[e]);
     }
 };
 
 // NV vectors a lane of the part of a row that starts at vector j0 (lane stride: NT vectors,
 // so a wave's load covers 1 KB without a gap).  Parts without a row's end in them take the
-// branch with plain loads.
+// branch with plain loads, from one address and an offset a lane.
+template <typename T, int NT, int NV>
+__device__ __forceinline__ bool inside(const Row<T>& row, int j0) {
+    return row.whole(j0) && row.whole(j0 + NT * NV - 1);
+}
 template <typename T, int NT, int NV>
 __device__ __forceinline__ void load_part(const Row<T>& row, int j0, uint4 (&raw)[NV]) {
-    if (row.whole(j0) && row.whole(j0 + NT * NV - 1)) {
+    if (inside<T, NT, NV>(row, j0)) {
+        const char* p = row.base + row.col(j0) * T::kSize;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) raw[i] = row.load_whole(j0 + i * NT + (int)threadIdx.x);
+        for (int i = 0; i < NV; ++i) raw[i] = *(const uint4*)(p + i * NT * 16 + threadIdx.x * 16u);
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) raw[i] = row.load(j0 + i * NT + (int)threadIdx.x);
+    }
+}
+// The same part of another row (gradients): value(i, f) gives vector i, without(i) the bits of entries
+// that are not to be written.
+template <typename T, int NT, int NV, class Value, class Without>
+__device__ __forceinline__ void store_part(const Row<T>& row, char* out, int j0, Value value, Without without) {
+    const bool plain = inside<T, NT, NV>(row, j0) && (((uintptr_t)out ^ (uintptr_t)row.base) & 15) == 0;
+    char* p = out + row.col(j0) * T::kSize;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float f[T::kVec];
+        value(i, f);
+        const uint32_t skip = without(i);
+        if (plain && !__any(skip != 0))
+            *(uint4*)(p + i * NT * 16 + threadIdx.x * 16u) = pack(f, T());
+        else
+            row.store(out, j0 + i * NT + (int)threadIdx.x, f, skip);
     }
 }
 
@@ -162,7 +185,7 @@ __device__ __forceinline__ uint4 again(uint4 r) {
 }
 
 // A part's softmax: with d_i = (x_i - m) log2(e) / T over its entries, s = sum 2^d_i and
-// u = sum 2^d_i d_i.  m starts at the lowest finite value, so that -inf entries (d = -inf)
+// u = sum 2^d_i d_i, for a reference m near its maximum.  m starts at the lowest finite value, so that -inf entries (d = -inf)
 // add nothing and a part of them alone has s = 0; NaN and +inf make s NaN for good.
 struct Part {
     float m, s, u;
@@ -171,44 +194,47 @@ __device__ __forceinline__ Part no_part() { return Part{-FLT_MAX, 0.0f, 0.0f}; }
 
 // A lane's own running sums, an entry in four operations and the exponential.  d is one fused
 // product, x log2(e) / T - scaled, with scaled = m log2(e) / T as float32 has it; what scaled lost in
-// rounding (`lost`) is given back at the end (part_of), exactly.  That needs scaled to be known to
-// a small part of one, so where it is over kWide (logits in the millions; rows masked by the type's
-// lowest value and little else) d is (x - m) log2(e) / T instead, for the waves that have such lanes.
+// rounding (`lost`) is given back at the end (part_of), exactly.  m is a reference, not the maximum: it
+// follows when an entry exceeds it by 8 binary orders (limit), which after a lane's first vector is
+// seldom, and a sum of 2^8 is as exact as one of 1.
+// scaled has to be known to a small part of one, so where it is over kWide (logits in the millions;
+// rows masked by the type's lowest value and little else) d is (x - m) log2(e) / T instead, for the
+// waves that have such lanes: their limit is -inf.
 constexpr float kWide = 1048576.0f;
 struct Lane {
-    float m, scaled, wide;      // wide: entries from here on need the other form; +inf: none do
-    float s, u;
+    float m, scaled, limit, s, u;
 };
-__device__ __forceinline__ Lane no_lane() { return Lane{-FLT_MAX, -3e38f, INFINITY, 0.0f, 0.0f}; }
+__device__ __forceinline__ Lane no_lane() { return Lane{-FLT_MAX, -3e38f, -INFINITY, 0.0f, 0.0f}; }
 __device__ __forceinline__ float lost(const Lane& l, float c) {
     return fabsf(l.scaled) > kWide ? 0.0f : -fmaf(l.m, c, -l.scaled);                       // scaled - m c
 }
 template <bool ENTROPY, int N>
 __device__ __forceinline__ void add_vector(Lane& l, const float (&f)[N], float most, float c) {
-    if (__any(most > l.m || (most == l.m && l.s == 0.0f))) {
+    if (__any(most > l.limit)) {
         Lane to = l;
-        to.m = fmaxf(l.m, most);
-        to.scaled = fminf(fmaxf(to.m * c, -3e38f), 3e38f);
-        float d = l.scaled - to.scaled;
-        if (__any(fabsf(l.scaled) > kWide || fabsf(to.scaled) > kWide)) {
-            d = (l.m - to.m) * c + (lost(l, c) - lost(to, c));
-            to.wide = fabsf(to.scaled) > kWide && (most >= -FLT_MAX || l.m > -FLT_MAX) ? -FLT_MAX : INFINITY;
+        if (most > l.limit) {
+            to.m = fmaxf(l.m, most);
+            to.scaled = fminf(fmaxf(to.m * c, -3e38f), 3e38f);
+            to.limit = fabsf(to.scaled) > kWide ? -INFINITY : to.m + 8.0f / c;
         }
+        float d = l.scaled - to.scaled;
+        if (__any(fabsf(l.scaled) > kWide || fabsf(to.scaled) > kWide))
+            d = (l.m - to.m) * c + (lost(l, c) - lost(to, c));
         d = fmaxf(d, kDead);
         const float r = __builtin_amdgcn_exp2f(d);
         if (ENTROPY) to.u = r * fmaf(l.s, d, l.u);
         to.s = l.s * r;
         l = to;
-    }
-    if (__any(most >= l.wide)) {
+        if (__any(fabsf(l.scaled) > kWide && most >= -FLT_MAX)) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float d = l.wide < 0.0f ? (f[e] - l.m) * c : fmaf(f[e], c, -l.scaled);
-            const float w = __builtin_amdgcn_exp2f(d);
-            l.s += w;
-            if (ENTROPY) l.u = fmaf(w, fmaxf(d, kDead), l.u);
+            for (int e = 0; e < N; ++e) {
+                const float d = fabsf(l.scaled) > kWide ? (f[e] - l.m) * c : fmaf(f[e], c, -l.scaled);
+                const float w = __builtin_amdgcn_exp2f(d);
+                l.s += w;
+                if (ENTROPY) l.u = fmaf(w, fmaxf(d, kDead), l.u);
+            }
+            return;
         }
-        return;
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -314,18 +340,6 @@ void with_part_shape(const Shape& s, F f) {
     DDM_SHAPE(256, 4);
     DDM_SHAPE(256, 8);
 }
-template <typename F>
-void with_row_shape(const Shape& s, F f) {
-    DDM_SHAPE(64, 1);
-    DDM_SHAPE(64, 2);
-    DDM_SHAPE(64, 4);
-    DDM_SHAPE(64, 8);
-    DDM_SHAPE(256, 4);
-    DDM_SHAPE(256, 8);
-    DDM_SHAPE(1024, 4);
-    DDM_SHAPE(1024, 8);
-    DDM_SHAPE(1024, 16);
-}
 #undef DDM_SHAPE
 
 // The checks the entry points share; 0 or DDM_E_ARG with the reason.
@@ -333,7 +347,7 @@ inline int check_rows(const char* who, int32_t dtype, int64_t n, int64_t v, int6
                       float temperature, int32_t top) {
     if (dtype != DDM_F32 && dtype != DDM_BF16 && dtype != DDM_F16) {
         set_error("%s: unknown type %d", who, (int)dtype);
-    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts) {
+    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts - 8) {
         set_error("%s: invalid argument (rows %lld, columns %lld of 1..%lld, row stride %lld)", who, (long long)n,
                   (long long)v, (long long)kMaxColumns, (long long)ld);
     } else if (target_bytes != 4 && target_bytes != 8) {

@@ -2,7 +2,7 @@
 // flag and the top alternatives of every row of logits, in one pass over them; and the
 // gradient of weighted log probabilities, entropies and alternatives.
 //
-// With d_i = (x_i - m) / T, m the row's maximum, S = sum e^d_i, U = sum e^d_i d_i:
+// With d_i = (x_i - m) / T, m near the row's maximum, S = sum e^d_i, U = sum e^d_i d_i:
 //   log p_i = d_i - log S,   H = log S - U / S,   rank = #{x_i > x_t or x_i = x_t, i < t}.
 // The pass is bound by reading the logits; what it computes per entry (about 13 vector
 // operations, one of them an exponential at a quarter of the rate) is just under what hides
@@ -177,7 +177,7 @@ __device__ __forceinline__ void select_top(SelectLds& l, uint32_t best, int k, i
 }
 
 // ---- one row's results -------------------------------------------------------------------------
-// What is common to a row: its maximum, log S (0 for a row with nothing left, NaN for a row
+// What is common to a row: its reference (see Part), log S (0 for a row with nothing left, NaN for a row
 // with NaN or +inf in it).
 struct RowLog {
     float m, log_s;
@@ -241,6 +241,8 @@ __global__ __launch_bounds__(NT) void k_score_parts(ScoreArgs a) {
     const Row<T> row(a.x + r * a.ld_bytes, a.v);
     const int turns = a.turns, j0 = part * NT * NV * turns;
 
+    uint4 raw[NV];
+    load_part<T, NT, NV>(row, j0, raw);                  // under way while the target is looked up
     const float c = kLog2e / a.temperature;
     const int64_t t = target_at(a.target, a.target_wide, r);
     const bool counts = t >= 0 && t < a.v;
@@ -256,8 +258,7 @@ __global__ __launch_bounds__(NT) void k_score_parts(ScoreArgs a) {
     uint32_t ahead = 0;
     for (int turn = 0; turn < turns; ++turn) {
         const int jt = j0 + turn * NT * NV;
-        uint4 raw[NV];
-        load_part<T, NT, NV>(row, jt, raw);
+        if (turn) load_part<T, NT, NV>(row, jt, raw);
         float turn_most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -419,14 +420,14 @@ __global__ __launch_bounds__(NT) void k_score_grad(GradArgs a) {
         const float d = (x - m) * c - log2_s;
         return dead ? 0.0f : __builtin_amdgcn_exp2f(d) * fmaf(B, fmaxf(d, kDead), A);
     };
+    store_part<T, NT, NV>(
+        row, out, j0,
+        [&](int i, float (&f)[T::kVec]) {
+            unpack(raw[i], f, T());
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float f[T::kVec];
-        unpack(raw[i], f, T());
-#pragma unroll
-        for (int e = 0; e < T::kVec; ++e) f[e] = value(f[e]);
-        row.store(out, j0 + i * NT + (int)threadIdx.x, f);
-    }
+            for (int e = 0; e < T::kVec; ++e) f[e] = value(f[e]);
+        },
+        [](int) { return 0u; });
     __syncthreads();
     auto put = [&](int col, float x, float extra) {
         T::store(out + col * T::kSize, dead ? 0.0f : fmaf(extra, inv_t, value(x)));
@@ -447,7 +448,7 @@ inline Shape shape_of(int64_t n, int64_t nvec, bool turns) {
         s.nv = nvec <= 64 ? 1 : nvec <= 128 ? 2 : nvec <= 256 ? 4 : 8;
     } else {
         while (s.nv > 1 && n * ceil_div(nvec, 256 * s.nv) < 1024 && ceil_div(nvec, 128 * s.nv) <= kMaxParts) s.nv /= 2;
-        while (turns && s.turns < 4 && n * ceil_div(nvec, 256 * s.nv * s.turns * 2) >= 4096) s.turns *= 2;
+        while (turns && s.turns < 4 && n * ceil_div(nvec, 256 * s.nv * s.turns * 2) >= 8192) s.turns *= 2;
     }
     s.parts = (int)ceil_div(nvec, (int64_t)s.nt * s.nv * s.turns);
     return s;

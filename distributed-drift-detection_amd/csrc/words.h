@@ -1,0 +1,44 @@
+// What workgroups of one launch tell each other: 8-byte words of two float32, one store each, which
+// are their own sign of having been written (unset words hold all ones), so no fence is needed.
+// Work that waits is taken by tickets, so that what it waits for already runs or starts next.
+#pragma once
+#include "common.h"
+
+namespace ddm {
+
+constexpr uint64_t kUnset = ~0ull;
+constexpr uint32_t kSpinLimit = 1u << 22;      // some seconds: a guard, not a wait
+
+__device__ __forceinline__ uint64_t word(float a, float b) {
+    const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    return w == kUnset ? w ^ 1u : w;               // two NaN of all ones: another NaN
+}
+__device__ __forceinline__ float word_a(uint64_t w) { return __uint_as_float((uint32_t)w); }
+__device__ __forceinline__ float word_b(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
+__device__ __forceinline__ void publish(uint64_t* p, uint64_t w) {
+    __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Queues of tickets: one counter gives out a ticket every 15 ns (measured: 32768 workgroups that took
+// one each ran no faster than that), so a launch has up to 8, 256 bytes apart, and a workgroup takes
+// from the queue that its index says.  What waits for each other is given out by one queue.
+constexpr int kQueues = 8;
+constexpr int64_t kTicketBytes = kQueues * 256;
+struct Ticket {
+    uint32_t queue, number;     // the same in every lane, and known to be
+};
+__device__ __forceinline__ Ticket take_ticket(uint32_t* tickets, uint32_t queues) {
+    __shared__ uint32_t sh;
+    const uint32_t q = blockIdx.x & (queues - 1u);
+    if (threadIdx.x == 0) sh = atomicAdd(tickets + q * 64, 1u);
+    __syncthreads();
+    return Ticket{q, (uint32_t)__builtin_amdgcn_readfirstlane(sh)};
+}
+
+// Before such a launch: tickets 0, words unset; and what is copied on the way (from NULL: zeros).
+int reset_words(uint32_t* tickets, uint64_t* words, int64_t nwords, const float* from, float* to, int64_t ncopy,
+                hipStream_t stream, const char* who);
+
+}  // namespace ddm

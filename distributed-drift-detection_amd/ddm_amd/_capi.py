@@ -156,7 +156,7 @@ SIGNATURES = {
                                         _vp, _vp, _vp, _vp, _vp, _vp]),
     "ddm_token_scores_grad": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _vp,
                                              _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
-    "ddm_topk_distill_scratch_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32]),
+    "ddm_topk_distill_scratch_bytes": (_i64, [_i64, _i64, _i32]),
     "ddm_topk_distill": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32, _f32, _vp, _vp, _vp,
                                         _i64, _vp, _vp, _vp, _vp]),
     "ddm_gated_scan_scratch_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),

@@ -223,7 +223,7 @@ def topk_distill(logits, index, logprob, tail="rest", temperature=1.0, weight=No
         index, logprob, weight = dense(index), dense(logprob), dense(weight)
         loss = torch.empty(n, dtype=torch.float32, device=logits.device)
         out = _new_like(out, logits) if grad or out is not None else None
-        need = int(lib.ddm_topk_distill_scratch_bytes(n, v, code, k, out is not None))
+        need = int(lib.ddm_topk_distill_scratch_bytes(n, v, code))
         scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
         out_ld = v if out is None or n <= 1 else out.stride(0)
         check(lib.ddm_topk_distill(logits.data_ptr(), code, n, v, ld, index.data_ptr(), index.element_size(),

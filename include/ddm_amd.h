@@ -750,7 +750,7 @@ int ddm_forest_predict_dev(const ddm_predict_segment* segs_dev, const int64_t* c
  *   rank[n]    entries before the target in the order (value descending, column ascending)
  *   err[ceil16(n)]  1: the target is not the first alternative (rank > 0, or masked), else 0;
  *              the bytes behind row n - 1 are zeroed, so the scans can read whole words
- *   stats[2n]  (maximum, log2 of the sum) for ddm_token_scores_grad
+ *   stats[2n]  (a reference near the maximum, log2 of the sum) for ddm_token_scores_grad
  *   top_logprob[n * top], top_index[n * top]  the `top` (0..64) largest, in that order
  * A target outside [0, v) is not scored: logprob 0, rank -1, err 0.  -inf entries are masked:
  * never an alternative (index -1, logprob -inf behind the last), probability 0.  A row of them
@@ -783,11 +783,11 @@ int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t n, int64_t 
  * is given (renorm), NaN for a row with NaN or +inf.  grad (NULL: the loss alone): the gradient
  * of sum weight loss (weight[n], NULL: 1) in the logits' type, row stride grad_ld; the logits'
  * own buffer with their stride, or one apart from it.  Rows of weight 0, and rows of -inf alone,
- * have gradient 0.  scratch: ddm_topk_distill_scratch_bytes(...) bytes, 16-byte aligned (NULL
- * if 0). */
+ * have gradient 0.  scratch: ddm_topk_distill_scratch_bytes(...) bytes, 16-byte aligned, for
+ * one call at a time (NULL if 0). */
 #define DDM_TAIL_RENORM 0
 #define DDM_TAIL_REST   1
-int64_t ddm_topk_distill_scratch_bytes(int64_t n, int64_t v, int32_t dtype, int32_t k, int32_t grad);
+int64_t ddm_topk_distill_scratch_bytes(int64_t n, int64_t v, int32_t dtype);
 int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld, const void* index,
                      int32_t index_bytes, const float* logprob, int32_t k, int32_t tail, float temperature,
                      const float* weight, float* loss, void* grad, int64_t grad_ld, void* scratch,

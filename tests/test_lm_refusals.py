@@ -111,8 +111,8 @@ def test_distill_entry_point_checks_before_it_launches():
                      ({"index": None}, "null"), ({"grad": one, "grad_ld": 9}, "gradient stride"),
                      ({"v": 100000, "ld": 100000}, "null")):
         assert distill(**kw) == _capi.DDM_E_ARG and text in last_error(), (kw, last_error())
-    assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100, 0, 3, 1) == 0
-    assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100000, 0, 3, 1) > 0
+    assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100, 0) == 0
+    assert _capi.lib.ddm_topk_distill_scratch_bytes(4, 100000, 0) > 0
 
 
 G = torch.zeros(4, 5)
