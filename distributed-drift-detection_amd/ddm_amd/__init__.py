@@ -23,5 +23,6 @@ _EXPORTS = {
 
 def __getattr__(name):
     if name in _EXPORTS:
-        return getattr(importlib.import_module(f".{_EXPORTS[name]}", __name__), name)
+        value = globals()[name] = getattr(importlib.import_module(f".{_EXPORTS[name]}", __name__), name)
+        return value                                    # found as a plain attribute from now on
     raise AttributeError(name)

@@ -13,8 +13,8 @@ nothing back and can be captured; results do not change from run to run.
 import torch
 
 from ._capi import check, lib
+from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, shaped
 from .kernels import _evs, _ptr
-from .tokens import DTYPES, launch_on, overlap, rows_of, shaped
 
 SCALES = {"none": 0, "ewma": 1, "unit": 2}
 
@@ -57,15 +57,6 @@ def _sequences(offsets, state, name, d):
     return n
 
 
-def _own(t):
-    return None if t is None else t.contiguous()
-
-
-def _scratch(rows, d, gates, code, grad, device):
-    need = int(lib.ddm_gated_scan_scratch_bytes(rows, d, gates, code, grad))
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-
-
 def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, stream=None, timer=None):
     """h [rows, d] (x's type) and the state after every sequence [n, d] (float32) of
     h_t = exp(log_a_t) h_{t-1} + b_t, b = x ("none"), (1 - a) x ("ewma") or sqrt(1 - a^2) x ("unit").
@@ -89,11 +80,12 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
                 raise ValueError("out overlaps an input without being x")
     else:
         ld_out = d
-    with launch_on(x, stream, (x, log_a, offsets, state, out)) as s:
-        offsets, state = _own(offsets), _own(state)
+    context, s = launch_on(x, stream, (x, log_a, offsets, state, out))
+    with context:
+        offsets, state = dense(offsets), dense(state)
         h = torch.empty((rows, d), dtype=x.dtype, device=x.device) if out is None else out
         after = torch.empty((n, d), dtype=torch.float32, device=x.device)
-        scratch = _scratch(rows, d, gates, DTYPES[x.dtype], 0, x.device)
+        scratch = scratch_for(x.device, "ddm_gated_scan_scratch_bytes", rows, d, gates, DTYPES[x.dtype], 0)
         check(lib.ddm_gated_scan(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a, rows,
                                  d, gates, _ptr(offsets), n, mode, _ptr(state), after.data_ptr(), h.data_ptr(), ld_out,
                                  out is None, _ptr(scratch), s, *_evs(timer)), "ddm_gated_scan")
@@ -115,12 +107,13 @@ def gated_scan_grad(x, log_a, h, d_h, offsets=None, state=None, d_state=None, sc
             raise ValueError(f"{name} must be {x.dtype} {list(x.shape)}, got {t.dtype} {list(t.shape)}")
     if d_state is not None:
         shaped("d_state", d_state, (n, d), torch.float32)
-    with launch_on(x, stream, (x, log_a, h, d_h, offsets, state, d_state)) as s:
-        offsets, state, d_state = _own(offsets), _own(state), _own(d_state)
+    context, s = launch_on(x, stream, (x, log_a, h, d_h, offsets, state, d_state))
+    with context:
+        offsets, state, d_state = dense(offsets), dense(state), dense(d_state)
         d_x = torch.empty((rows, d), dtype=x.dtype, device=x.device)
         d_a = torch.empty((rows, gates), dtype=log_a.dtype, device=x.device)
         before = torch.empty((n, d), dtype=torch.float32, device=x.device)
-        scratch = _scratch(rows, d, gates, DTYPES[x.dtype], 1, x.device)
+        scratch = scratch_for(x.device, "ddm_gated_scan_scratch_bytes", rows, d, gates, DTYPES[x.dtype], 1)
         check(lib.ddm_gated_scan_grad(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a,
                                       h.data_ptr(), strides[0], d_h.data_ptr(), strides[1], rows, d, gates,
                                       _ptr(offsets), n, mode, _ptr(state), _ptr(d_state), before.data_ptr(),
@@ -142,7 +135,8 @@ def gated_step(x, log_a, state=None, scale="none", out_state=None, stream=None, 
     if state is not None and out_state is not None and state.data_ptr() != out_state.data_ptr() and \
             overlap(state, out_state):
         raise ValueError("out_state overlaps the state without being it")
-    with launch_on(x, stream, (x, log_a, state, out_state)) as s:
+    context, s = launch_on(x, stream, (x, log_a, state, out_state))
+    with context:
         h = torch.empty((rows, d), dtype=x.dtype, device=x.device)
         after = torch.empty((rows, d), dtype=torch.float32, device=x.device) if out_state is None else out_state
         check(lib.ddm_gated_step(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a, rows,

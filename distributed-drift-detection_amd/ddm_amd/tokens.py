@@ -10,14 +10,13 @@ The calls are asynchronous on `stream` (default: the current stream of the logit
 read nothing back and can be captured.  Results belong to that stream.
 """
 import collections
-import ctypes
 
 import torch
 
 from ._capi import check, lib
+from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, shaped
 from .kernels import _evs, _ptr
 
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_COLUMNS = 1 << 19
 MAX_TOP = 64
 
@@ -26,73 +25,6 @@ TokenScores = collections.namedtuple("TokenScores", ["logprob", "entropy", "rank
 TokenScores.__doc__ = """What token_scores returns: logprob, entropy float32 [n]; rank int32 [n]; err uint8
 [n rounded up to 16] (the scans' layout, zeros behind row n-1); top_logprob float32 and top_index int32 [n, top]
 (None for top 0); stats float32 [n, 2] and the temperature, for token_scores_grad."""
-
-
-class launch_on:
-    """The device of `t` and the stream to launch on, as a context: what is allocated inside
-    belongs to that stream, and inputs stay alive for it."""
-
-    def __init__(self, t, stream, inputs):
-        if t.device.type != "cuda":
-            raise ValueError(f"tensors must be on the GPU, got {t.device}")
-        for x in inputs:
-            if x is not None and x.device != t.device:
-                raise ValueError(f"tensors on {t.device} and on {x.device}")
-        current = torch.cuda.current_stream(t.device)
-        self.stream = stream if stream is not None else current
-        if self.stream.device != t.device:
-            raise ValueError(f"stream of {self.stream.device}, tensors on {t.device}")
-        if self.stream != current:
-            for x in inputs:
-                if x is not None:
-                    x.record_stream(self.stream)
-        self.ctx = torch.cuda.stream(self.stream)
-
-    def __enter__(self):
-        self.ctx.__enter__()            # also makes the stream's device the current one
-        return ctypes.c_void_p(self.stream.cuda_stream)
-
-    def __exit__(self, *exc):
-        return self.ctx.__exit__(*exc)
-
-
-def rows_of(name, t, dtypes=DTYPES):
-    """The row stride of a matrix whose rows are contiguous."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.dim() != 2:
-        raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} has type {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}'s rows must be contiguous (strides {t.stride()})")
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        raise ValueError(f"{name}'s rows overlap (strides {t.stride()})")
-    return ld
-
-
-def shaped(name, t, shape, *dtypes):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes:
-        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} {list(shape)}, got {t.dtype} "
-                         f"{list(t.shape)}")
-
-
-def dense(t):
-    """`t` without gaps (a copy on the launch stream if it has any)."""
-    return None if t is None else t.contiguous()
-
-
-def _span(t):
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-
-def overlap(a, b):
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
 
 
 def _temperature(t):
@@ -139,21 +71,22 @@ def token_scores(logits, targets, top=0, temperature=1.0, stream=None, timer=Non
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top must be 0..{MAX_TOP}, got {top}")
     dev, code = logits.device, DTYPES[logits.dtype]
-    with launch_on(logits, stream, (logits, targets)) as s:
+    context, s = launch_on(logits, stream, (logits, targets))
+    with context:
         targets = dense(targets)
-        f32 = torch.empty((4, n), dtype=torch.float32, device=dev)
-        logprob, entropy, stats = f32[0], f32[1], f32[2:].view(-1)
+        logprob = torch.empty(n, dtype=torch.float32, device=dev)
+        entropy = torch.empty_like(logprob)
+        stats = logprob.new_empty((n, 2))
         rank = torch.empty(n, dtype=torch.int32, device=dev)
         err = torch.empty((n + 15) // 16 * 16, dtype=torch.uint8, device=dev)
-        top_lp = torch.empty((n, top), dtype=torch.float32, device=dev) if top else None
-        top_ix = torch.empty((n, top), dtype=torch.int32, device=dev) if top else None
-        need = int(lib.ddm_token_scores_scratch_bytes(n, v, code, top))
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        top_lp = logprob.new_empty((n, top)) if top else None
+        top_ix = rank.new_empty((n, top)) if top else None
+        scratch = scratch_for(dev, "ddm_token_scores_scratch_bytes", n, v, code, top)
         check(lib.ddm_token_scores(logits.data_ptr(), code, n, v, ld, targets.data_ptr(), targets.element_size(),
                                    temperature, top, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                    rank.data_ptr(), err.data_ptr(), _ptr(top_lp), _ptr(top_ix), _ptr(scratch), s,
                                    *_evs(timer)), "ddm_token_scores")
-    return TokenScores(logprob, entropy, rank, err, top_lp, top_ix, stats.view(n, 2), temperature)
+    return TokenScores(logprob, entropy, rank, err, top_lp, top_ix, stats, temperature)
 
 
 def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d_top=None, out=None, stream=None,
@@ -178,7 +111,8 @@ def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d
         shaped("d_top", d_top, (n, top), torch.float32)
     _check_out(out, logits)
     given = (logits, targets, scores.stats, scores.entropy, index, d_logprob, d_entropy, d_top, out)
-    with launch_on(logits, stream, given) as s:
+    context, s = launch_on(logits, stream, given)
+    with context:
         targets, stats, entropy, index, d_logprob, d_entropy, d_top = map(dense, given[1:8])
         out = _new_like(out, logits)
         out_ld = out.stride(0) if n > 1 else v
@@ -219,12 +153,12 @@ def topk_distill(logits, index, logprob, tail="rest", temperature=1.0, weight=No
         shaped("weight", weight, (n,), torch.float32)
     _check_out(out, logits)
     code = DTYPES[logits.dtype]
-    with launch_on(logits, stream, (logits, index, logprob, weight, out)) as s:
+    context, s = launch_on(logits, stream, (logits, index, logprob, weight, out))
+    with context:
         index, logprob, weight = dense(index), dense(logprob), dense(weight)
         loss = torch.empty(n, dtype=torch.float32, device=logits.device)
         out = _new_like(out, logits) if grad or out is not None else None
-        need = int(lib.ddm_topk_distill_scratch_bytes(n, v, code))
-        scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+        scratch = scratch_for(logits.device, "ddm_topk_distill_scratch_bytes", n, v, code)
         out_ld = v if out is None or n <= 1 else out.stride(0)
         check(lib.ddm_topk_distill(logits.data_ptr(), code, n, v, ld, index.data_ptr(), index.element_size(),
                                    logprob.data_ptr(), k, TAILS[tail], temperature, _ptr(weight), loss.data_ptr(),
