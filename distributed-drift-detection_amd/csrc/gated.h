@@ -84,7 +84,7 @@ struct Args {
     int cl_bits, ncb, group;             // lanes across channels (log2), channel blocks, tiles a group
     int64_t ntiles;
     uint32_t *tickets, queues;            // NULL: one tile, no chain
-    uint64_t *agg, *inc;                  // [ntiles][dp], [groups][dp]
+    uint64_t *agg, *inc, *far;            // [ntiles][dp], [groups][dp], [groups / 64][dp]
     int64_t dp;
     float* dl_part;                       // [rows][parts a row] or NULL: dl itself
     int dl_width;                         // lanes summed within a wave
@@ -102,19 +102,18 @@ __device__ __forceinline__ Step after(const Step& p, const Step& q) {   // p, th
 __device__ __forceinline__ float apply(const Step& s, float h) { return s.a < 0.0f ? s.b : fmaf(s.a, h, s.b); }
 
 // ---- gates ---------------------------------------------------------------------------------------
-// 1 - e^y without cancellation, given e = e^y: a series up to |y| = 0.7 (the first term left out
-// is under 2^-26 of the result), the difference beyond, where e is at most half.
+// 1 - e^y without cancellation, given e = e^y: for |y| <= 0.5 by (e^y - 1) / y, interpolated there in
+// seven Chebyshev points (within 1.2 half steps, rounding included), beyond as the difference, where
+// e is under 0.61.
 __device__ __forceinline__ float one_minus_exp(float y, float e) {
-    float p = 2.7557319e-6f;                        // 1/9!
-    p = fmaf(p, y, 2.4801587e-5f);
-    p = fmaf(p, y, 1.9841270e-4f);
-    p = fmaf(p, y, 1.3888889e-3f);
-    p = fmaf(p, y, 8.3333333e-3f);
-    p = fmaf(p, y, 4.1666667e-2f);
-    p = fmaf(p, y, 1.6666667e-1f);
-    p = fmaf(p, y, 0.5f);
+    float p = 1.996217616e-4f;
+    p = fmaf(p, y, 1.399777364e-3f);
+    p = fmaf(p, y, 8.333181962e-3f);
+    p = fmaf(p, y, 4.166530445e-2f);
+    p = fmaf(p, y, 1.666666716e-1f);
+    p = fmaf(p, y, 0.5000000596f);
     p = fmaf(p, y, 1.0f);
-    return fabsf(y) <= 0.7f ? -y * p : 1.0f - e;
+    return fabsf(y) <= 0.5f ? -y * p : 1.0f - e;
 }
 // a = e^l and the input's factor.  The exponential's argument is rounded once: half a step for each
 // binary order that a loses, which is less the less a weighs.
@@ -125,9 +124,8 @@ template <int SCALE>
 __device__ __forceinline__ Gate gate_of(float l) {
     Gate g;
     g.a = __builtin_amdgcn_exp2f(l * 1.4426950408889634f);
-    g.f = SCALE == DDM_GATED_NONE   ? 1.0f
-          : SCALE == DDM_GATED_EWMA ? one_minus_exp(l, g.a)
-                                    : __builtin_amdgcn_sqrtf(fmaxf(one_minus_exp(2.0f * l, g.a * g.a), 0.0f));
+    g.f = SCALE == DDM_GATED_NONE ? 1.0f : one_minus_exp(l, g.a);
+    if (SCALE == DDM_GATED_UNIT) g.f = __builtin_amdgcn_sqrtf(fmaxf(fmaf(g.f, g.a, g.f), 0.0f));    // (1 - a)(1 + a)
     return g;
 }
 // The factor's derivative by l.
@@ -155,11 +153,12 @@ struct Place {
     int block;             // of channels
 };
 __device__ __forceinline__ Place take(const Args& a) {
-    if (!a.tickets) return Place{(int64_t)(blockIdx.x / (uint32_t)a.ncb), (int)(blockIdx.x % (uint32_t)a.ncb)};
+    if (!a.tickets) return Place{0, (int)blockIdx.x};      // one tile
     // a queue gives out all tiles of every queues-th channel block, tile by tile
     const Ticket t = take_ticket(a.tickets, a.queues);
-    const uint32_t blocks = (uint32_t)a.ncb / a.queues;
-    return Place{(int64_t)(t.number / blocks), (int)(t.number % blocks * a.queues + t.queue)};
+    // (the division is the vector unit's; its result is the same in every lane)
+    const uint32_t blocks = (uint32_t)a.ncb / a.queues, tile = __builtin_amdgcn_readfirstlane(t.number / blocks);
+    return Place{(int64_t)tile, (int)((t.number - tile * blocks) * a.queues + t.queue)};
 }
 
 // Which rows of a tile begin and end a sequence: a bit a row, and the sequence's number where it is set.
@@ -178,14 +177,17 @@ struct Marks {
 };
 __device__ __forceinline__ void mark_rows(const Args& a, int64_t row0, int nrows, const Marks& m) {
     for (int i = threadIdx.x; i < nrows / 16; i += NT) m.begin_bits[i] = 0;     // and the end bits behind
-    int64_t lo = 0, hi = a.n;                       // the first sequence that ends behind row0
+    // the first sequence that ends behind row0, in one round of loads for up to 64 sequences, two for
+    // 4096: every lane looks at the last of its 64th of what is left
+    int64_t lo = 0, hi = a.n;
     while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (a.off[mid + 1] > row0)
-            hi = mid;
-        else
-            lo = mid + 1;
+        const int64_t step = (hi - lo + 63) / 64, i = lo + ((int64_t)(threadIdx.x & 63) + 1) * step - 1;
+        const int before = __popcll(__ballot(i < hi && a.off[i + 1] <= row0));     // lanes wholly before
+        lo += before * step;
+        if (step == 1) break;
+        hi = lo + step < hi ? lo + step : hi;
     }
+    if (lo > a.n) lo = a.n;
     __syncthreads();
     for (int64_t s = lo + threadIdx.x; s < a.n; s += NT) {
         const int64_t b = a.off[s], e = a.off[s + 1];
@@ -234,8 +236,67 @@ __device__ __forceinline__ void await(const uint64_t* p, int64_t stride, int cou
     }
 }
 
+__device__ __forceinline__ uint64_t await_one(const uint64_t* p) {
+    uint64_t w[1];
+    await<1>(p, 0, 1, w);
+    return w[0];
+}
+
+// The state before a tile, for one channel a thread, given the tile's own step.  Tiles form groups of
+// a.group; the last of a group publishes the state after it.
+__device__ __forceinline__ float carry_of_thread(const Args& a, int64_t tile, int64_t c, const Step& all) {
+    const int64_t g = tile / a.group;
+    const int in_group = (int)(tile % a.group);
+    const bool last = in_group == a.group - 1, more = tile + 1 < a.ntiles;
+    if (!last && more) publish(a.agg + tile * a.dp + c, word(all.a, all.b));
+    // the tiles before in the group first: they run beside this one; the group before is what
+    // there may be a wait for
+    Step sum{1.0f, 0.0f};
+    for (int j = 0; j < in_group; j += 8) {
+        uint64_t w[8];
+        await<8>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (j + i < in_group) sum = after(sum, Step{word_a(w[i]), word_b(w[i])});
+    }
+    const float carry = apply(sum, g > 0 ? word_a(await_one(a.inc + (g - 1) * a.dp + c)) : 0.0f);
+    if (last && more) publish(a.inc + g * a.dp + c, word(apply(all, carry), 0.0f));
+    return carry;
+}
+
+// The same for one channel a wave, where there are few: a lane for each tile before in the group, then
+// a lane for each group before (its step, published by its last tile), so nothing passes from group to
+// group one by one.  Every 64 groups the state itself is passed on.
+__device__ __forceinline__ Step wave_steps(const uint64_t* p, int64_t stride, int count) {
+    const int lane = threadIdx.x & 63;
+    Step s{1.0f, 0.0f};
+    if (lane < count) {
+        const uint64_t w = await_one(p + lane * stride);
+        s = Step{word_a(w), word_b(w)};
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const Step q{__shfl_down(s.a, d), __shfl_down(s.b, d)};
+        if ((lane & (2 * d - 1)) == 0) s = after(s, q);
+    }
+    return Step{__shfl(s.a, 0), __shfl(s.b, 0)};
+}
+__device__ __forceinline__ float carry_of_wave(const Args& a, int64_t tile, int64_t c, const Step& all) {
+    const int64_t g = tile / 64, h = g / 64;
+    const int in_group = (int)(tile % 64), in_groups = (int)(g % 64);
+    const bool first = (threadIdx.x & 63) == 0, last = in_group == 63, more = tile + 1 < a.ntiles;
+    if (first && !last && more) publish(a.agg + tile * a.dp + c, word(all.a, all.b));
+    const Step tiles = wave_steps(a.agg + g * 64 * a.dp + c, a.dp, in_group);
+    const Step group = after(tiles, all);
+    if (first && last && more) publish(a.inc + g * a.dp + c, word(group.a, group.b));
+    const Step groups = wave_steps(a.inc + h * 64 * a.dp + c, a.dp, in_groups);
+    const float carry = apply(tiles, apply(groups, h > 0 ? word_a(await_one(a.far + (h - 1) * a.dp + c)) : 0.0f));
+    if (first && last && in_groups == 63 && more) publish(a.far + h * a.dp + c, word(apply(all, carry), 0.0f));
+    return carry;
+}
+
 // From the steps of every lane's rows to the state before them: lanes of a wave by shuffles, the
-// waves and the tiles before by a thread for each channel.
+// waves and the tiles before by a thread (or a wave) for each channel.
 template <int VEC>
 __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step (&own)[VEC], ScanLds<VEC>& l,
                                       float (&h)[VEC]) {
@@ -266,39 +327,21 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
         }
     }
     __syncthreads();
-    if ((int)threadIdx.x < cols) {
-        const int col = threadIdx.x;
+    const bool waves = cols <= W;
+    const int col = waves ? wave : (int)threadIdx.x;
+    if (col < cols) {
         Step all{1.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < W; ++w) all = after(all, Step{l.a[w][col], l.b[w][col]});
         float carry = 0.0f;
         if (a.tickets) {
-            const int64_t c = (int64_t)at.block * cols + col, g = at.tile / a.group;
-            const int in_group = (int)(at.tile % a.group);
-            const bool last = in_group == a.group - 1, more = at.tile + 1 < a.ntiles;
-            if (!last && more) publish(a.agg + at.tile * a.dp + c, word(all.a, all.b));
-            // the tiles before in the group first: they run beside this one; the group before is
-            // what there may be a wait for
-            Step sum{1.0f, 0.0f};
-            for (int j = 0; j < in_group; j += 8) {
-                uint64_t w[8];
-                await<8>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (j + i < in_group) sum = after(sum, Step{word_a(w[i]), word_b(w[i])});
-            }
-            if (g > 0) {
-                uint64_t w[1];
-                await<1>(a.inc + (g - 1) * a.dp + c, 0, 1, w);
-                carry = word_a(w[0]);
-            }
-            carry = apply(sum, carry);
-            if (last && more) publish(a.inc + g * a.dp + c, word(apply(all, carry), 0.0f));
+            const int64_t c = (int64_t)at.block * cols + col;
+            carry = waves ? carry_of_wave(a, at.tile, c, all) : carry_of_thread(a, at.tile, c, all);
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             const float next = apply(Step{l.a[w][col], l.b[w][col]}, carry);
-            l.b[w][col] = carry;
+            if (!waves || lane == 0) l.b[w][col] = carry;
             carry = next;
         }
     }
@@ -342,7 +385,8 @@ struct Gates {
 struct Shape {
     int vec, cl_bits, ncb, r, group, dl_width, dl_parts;
     int64_t ntiles, dp;
-    int64_t words() const { return ntiles > 1 ? (ntiles + ceil_div(ntiles, group)) * dp : 0; }
+    int64_t words() const { return ntiles > 1 ? (ntiles + groups() + ceil_div(groups(), 64)) * dp : 0; }
+    int64_t groups() const { return ceil_div(ntiles, group); }
 };
 inline Shape shape_of(int64_t rows, int d, int share, int vec, bool grad) {
     Shape s;
@@ -355,7 +399,7 @@ inline Shape shape_of(int64_t rows, int d, int share, int vec, bool grad) {
     // rows a lane: many, so that a tile's share of the chain is small, unless that leaves CUs idle
     // or makes a tile's marks outgrow 34 KB of LDS
     s.r = grad ? 8 : 16;                              // four operands a row, not two
-    if (ceil_div(rows, tg * s.r) * s.ncb < 512 || tg * s.r > 4096) s.r = 4;
+    if (ceil_div(rows, tg * s.r) * s.ncb < 256 || tg * s.r > 4096) s.r = 4;
     s.ntiles = ceil_div(rows, (int64_t)tg * s.r);
     s.group = s.cl_bits == 6 ? 16 : 64;              // what a tile reads of others stays under a tenth of its own
     s.dp = (int64_t)(s.ncb << s.cl_bits) * vec;

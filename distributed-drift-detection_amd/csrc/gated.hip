@@ -156,6 +156,7 @@ int begin(Args& a, const Shape& s, void* scratch, const float* from, float* to, 
         a.queues = s.ncb % 8 == 0 ? 8 : s.ncb % 4 == 0 ? 4 : s.ncb % 2 == 0 ? 2 : 1;
         a.agg = (uint64_t*)(w + kTicketBytes);
         a.inc = a.agg + s.ntiles * s.dp;
+        a.far = a.inc + s.groups() * s.dp;
         w += kTicketBytes + 8 * words;
     }
     if (s.dl_parts) a.dl_part = (float*)w;

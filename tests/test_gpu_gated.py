@@ -273,3 +273,33 @@ def test_charts_of_a_models_scores():
                                scale="ewma")
     h2, _ = ddm_amd.gated_scan(signal[2000:], lam.expand(2000, 1), state=s1[1:], scale="ewma")
     close(h2, *(q[2000:] for q in ref["h"]))
+
+
+def test_a_stream_of_millions():
+    """Over 64 groups of 64 tiles of one channel; the reference's steps composed by doubling, in float64."""
+    import ddm_amd
+    rows = 8_600_007
+    gen = torch.Generator().manual_seed(6)
+    x = torch.rand(rows, 1, generator=gen)
+    lam = -torch.exp(torch.rand(rows, 1, generator=gen) * -7)
+    off = torch.tensor([0, 4_000_000, rows])
+    state = torch.tensor([[0.5], [0.25]])
+    h, after = ddm_amd.gated_scan(*on(x, lam, off, state), scale="ewma")
+    a, f = lam.double().exp().cuda(), (-torch.expm1(lam.double())).cuda()
+    b = f * x.double().cuda()
+    b[0] += a[0] * 0.5
+    b[4_000_000] += a[4_000_000] * 0.25
+    a[0] = a[4_000_000] = 0.0
+
+    def compose(a, b):
+        step = 1
+        while step < rows:
+            b = torch.cat([b[:step], b[step:] + a[step:] * b[:-step]])
+            a = torch.cat([a[:step], a[step:] * a[:-step]])
+            step *= 2
+        return b
+    want = compose(a, b).cpu()                      # everything is positive: the majorant is the state itself
+    tol = compose(a, 10 * 2.0 ** -24 * want.cuda()).cpu()
+    close(h, want, tol)
+    last = [3_999_999, rows - 1]
+    close(after, want[last], tol[last])
