@@ -7,7 +7,7 @@ namespace gated {
 // Rows in the opposite order: position p of the recurrence is row ntiles * tr - 1 - p, and a lane's
 // rows run from its last one back; bits of rows count from the first, as in the forward.
 template <typename X, typename L, int VEC, bool OWN, int R>
-__global__ __launch_bounds__(NT, 4) void k_gated_grad(Args a) {
+__global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
     const Place at = take(a);
