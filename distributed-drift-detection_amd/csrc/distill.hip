@@ -47,6 +47,12 @@ struct Kept {
     float l, x;                // teacher's log probability, student's logit
 };
 
+// The column of the thread's alternative; -1: none.
+__device__ __forceinline__ int column_of(const DistillArgs& a, int64_t r) {
+    if ((int)threadIdx.x >= a.k) return -1;
+    const int64_t i = target_at(a.index, a.index_wide, r * a.k + threadIdx.x);
+    return i >= 0 && i < a.v ? (int)i : -1;
+}
 template <typename T>
 __device__ __forceinline__ Kept load_kept(const DistillArgs& a, int64_t r, int col, const Row<T>& row) {
     const int lane = threadIdx.x & 63;
@@ -208,11 +214,7 @@ __global__ __launch_bounds__(NT) void k_distill(DistillArgs a) {
     uint4 raw[NV];
     load_part<T, NT, NV>(row, j0, raw);
     const float c = kLog2e / a.temperature;
-    int col = -1;
-    if ((int)threadIdx.x < a.k) {
-        const int64_t i = target_at(a.index, a.index_wide, r * a.k + threadIdx.x);
-        col = i >= 0 && i < a.v ? (int)i : -1;
-    }
+    const int col = column_of(a, r);
     mark_kept<NT, NV>(bits, col >= 0, col >= 0 ? row.vector_of(col) - j0 : -1, (col + row.head) % T::kVec);
     Kept k{-1, 0.0f, 0.0f};
     const bool finish = part == 0 && threadIdx.x < 64;
@@ -256,6 +258,41 @@ __global__ __launch_bounds__(NT) void k_distill(DistillArgs a) {
         },
         [&](int i) { return (uint32_t)((const uint8_t*)bits)[i * NT + threadIdx.x]; });
     if (finish && k.col >= 0) T::store(out + k.col * T::kSize, kept_grad);
+}
+
+// ---- the loss alone -----------------------------------------------------------------------------------
+// Nothing is to be written after the sums, so no part waits: a launch for the parts and one, a wave a
+// row, that joins them.
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT) void k_distill_parts(DistillArgs a) {
+    __shared__ uint32_t bits[NT * NV / 4];
+    __shared__ Part sh_part[NT / 64];
+    const int64_t r = blockIdx.x / (uint32_t)a.parts;
+    const int part = (int)(blockIdx.x % (uint32_t)a.parts), j0 = part * NT * NV;
+    const Row<T> row(a.x + r * a.ld_bytes, a.v);
+    uint4 raw[NV];
+    load_part<T, NT, NV>(row, j0, raw);
+    const float c = kLog2e / a.temperature;
+    if (a.rest) {
+        const int col = column_of(a, r);
+        mark_kept<NT, NV>(bits, col >= 0, col >= 0 ? row.vector_of(col) - j0 : -1, (col + row.head) % T::kVec);
+    }
+    const Part p = block_merge<NT>(sum_part<T, NT, NV>(raw, c, a.rest, bits), c, sh_part);
+    if (threadIdx.x == 0) a.words[blockIdx.x] = word(p.m, p.s);
+}
+template <typename T>
+__global__ __launch_bounds__(64) void k_distill_join(DistillArgs a) {
+    const int64_t r = blockIdx.x;
+    const Row<T> row(a.x + r * a.ld_bytes, a.v);
+    const Kept k = load_kept(a, r, column_of(a, r), row);
+    Part p = no_part();
+    if ((int)threadIdx.x < a.parts) {
+        const uint64_t w = a.words[r * a.parts + threadIdx.x];
+        p.m = word_a(w);
+        p.s = word_b(w);
+    }
+    float none;
+    finish_row<T>(a, r, k, wave_merge(p, kLog2e / a.temperature), none);
 }
 
 // A wave a row while the row fits its registers; 256 lanes and 8 vectors beyond, or fewer vectors
@@ -313,6 +350,15 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
             using T = decltype(type);
             DistillArgs a{(const char*)logits, n, v, ld * T::kSize, grad_ld * T::kSize, index, index_bytes == 8, logprob,
                           weight, k, tail == DDM_TAIL_REST, s.parts, temperature, loss, (char*)grad, nullptr, 1, nullptr};
+            if (s.parts > 1 && !grad) {
+                a.words = (uint64_t*)scratch;
+                with_part_shape(s, [&](auto nt, auto nv) {
+                    k_distill_parts<T, nt(), nv()><<<dim3((unsigned)(n * s.parts)), nt(), 0, st>>>(a);
+                });
+                if (int rc = launch_status("ddm_topk_distill")) return rc;
+                k_distill_join<T><<<dim3((unsigned)n), 64, 0, st>>>(a);
+                return launch_status("ddm_topk_distill");
+            }
             if (s.parts > 1) {
                 a.tickets = (uint32_t*)scratch;
                 while (a.queues < kQueues && a.queues * 2 * s.parts <= 128) a.queues *= 2;
