@@ -352,8 +352,8 @@ inline int check_rows(const char* who, int32_t dtype, int64_t n, int64_t v, int6
                   (long long)v, (long long)kMaxColumns, (long long)ld);
     } else if (target_bytes != 4 && target_bytes != 8) {
         set_error("%s: targets of %d bytes (4 or 8)", who, (int)target_bytes);
-    } else if (!(temperature > 0.0f) || !(temperature < INFINITY)) {
-        set_error("%s: temperature must be positive and finite", who);
+    } else if (!(temperature >= FLT_MIN) || !(temperature < INFINITY)) {
+        set_error("%s: temperature must be positive (a normal float32) and finite", who);
     } else if (top < 0 || top > kMaxTop) {
         set_error("%s: %d alternatives (0..%d)", who, (int)top, kMaxTop);
     } else {

@@ -29,8 +29,8 @@ TokenScores.__doc__ = """What token_scores returns: logprob, entropy float32 [n]
 
 def _temperature(t):
     t = float(t)
-    if not 0.0 < t < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {t}")
+    if not torch.finfo(torch.float32).tiny <= t < float("inf"):
+        raise ValueError(f"temperature must be positive (a normal float32) and finite, got {t}")
     return t
 
 

@@ -183,3 +183,24 @@ def test_refit_on_a_teachers_answers():
     want = distill64(teacher.float().cpu(), kept.top_index.cpu(), kept.top_logprob.cpu(), "rest", 1.0)
     close(same, want[0], want[1])
     close(flat, want[2], want[3])
+
+
+def test_calls_on_several_streams_at_once():
+    """Launches whose workgroups wait for each other, several in flight: each finishes, and is right."""
+    import ddm_amd
+    x, index, logprob = (t.cuda() for t in make(600, 60001, 20, torch.bfloat16, 9))
+    lam = -torch.rand(9000, 1024, device="cuda").bfloat16()
+    h_in = torch.randn(9000, 1024, device="cuda").bfloat16()
+    want = ddm_amd.topk_distill(x, index, logprob, grad=True)
+    want_h = ddm_amd.gated_scan(h_in, lam, scale="unit")
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            got.append(ddm_amd.gated_scan(h_in, lam, scale="unit", stream=s) if k % 2 else
+                       ddm_amd.topk_distill(x, index, logprob, grad=True, stream=s))
+    torch.cuda.synchronize()
+    for k, g in enumerate(got):
+        for a, b in zip(g, want_h if k % 2 else want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

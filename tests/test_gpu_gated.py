@@ -303,3 +303,26 @@ def test_a_stream_of_millions():
     close(h, want, tol)
     last = [3_999_999, rows - 1]
     close(after, want[last], tol[last])
+
+
+def test_beyond_four_gigabytes():
+    """Rows whose bytes lie past 2^32, forward and backward: a sequence there is what it is by itself."""
+    import ddm_amd
+    rows, d, first = 1_100_000, 2048, 1_090_000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(rows, d, dtype=B, device="cuda")
+    for r in range(0, rows, 110_000):
+        x[r:r + 110_000] = torch.randn(110_000, d, generator=gen, device="cuda")
+    lam = -torch.rand(rows, 16, generator=gen, device="cuda").to(B)
+    off = torch.tensor([0, first, rows], device="cuda")
+    h, s = ddm_amd.gated_scan(x, lam, offsets=off, scale="ewma")
+    few, fs = ddm_amd.gated_scan(x[first:], lam[first:], scale="ewma")
+    # tiles begin at other rows, so steps are composed in another order: float32's, then bf16's rounding
+    assert (s[1] - fs[0]).abs().max() < 1e-5
+    assert (h[first:].float() - few.float()).abs().max() < 2.0 ** -6
+    dx, dl, ds = ddm_amd.gated_scan_grad(x, lam, h, x, offsets=off, scale="ewma")
+    fx, fl, fd = ddm_amd.gated_scan_grad(x[first:], lam[first:], h[first:], x[first:], scale="ewma")
+    assert (ds[1] - fd[0]).abs().max() < 1e-4
+    assert (dx[first:].float() - fx.float()).abs().max() < 2.0 ** -4
+    assert (dl[first:].float() - fl.float()).abs().max() / fl.float().abs().max() < 2.0 ** -7
+

@@ -234,3 +234,46 @@ def test_scores_into_the_drift_scan(oracle_lib):
                          nb, ev, nev=nev, mode=1)
     want, _, _, _ = oracle_scan_c(oracle_lib, ref["err"].numpy(), np.array([0, n]), mode=1)
     assert np.array_equal(ev.cpu().numpy(), want) and (want[:, 1] >= 0).any()
+
+
+def test_beyond_four_gigabytes():
+    """Rows whose bytes lie past 2^32 score as the same rows by themselves."""
+    import ddm_amd
+    n, v = 33000, 70000
+    x = torch.empty(n, v, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for r in range(0, n, 11000):
+        x[r:r + 11000] = torch.randn(11000, v, generator=g, device="cuda") * 3
+    t = torch.randint(0, v, (n,), generator=g, device="cuda")
+    d = torch.randn(n, generator=g, device="cuda")
+    r = ddm_amd.token_scores(x, t, top=5)
+    dx = ddm_amd.token_scores_grad(x, t, r, d_logprob=d)
+    for a in (0, 15000, n - 40):
+        part, pt = x[a:a + 40], t[a:a + 40]
+        few = ddm_amd.token_scores(part, pt, top=5)
+        assert torch.equal(few.rank, r.rank[a:a + 40]) and torch.equal(few.top_index, r.top_index[a:a + 40])
+        # parts of another size sum in another order
+        assert (few.logprob - r.logprob[a:a + 40]).abs().max() < 1e-4
+        few_dx = ddm_amd.token_scores_grad(part, pt, few, d_logprob=d[a:a + 40])
+        assert (few_dx.float() - dx[a:a + 40].float()).abs().max() < 2.0 ** -7
+    ref = scores64(x[n - 3:].cpu(), t[n - 3:].cpu(), 5, 1.0)
+    assert torch.equal(r.rank[n - 3:].cpu(), ref["rank"])
+    close(r.logprob[n - 3:], ref["logprob"], scores_tolerance(x[:1].cpu(), ref, 1.0)[0](ref["logprob"]))
+
+
+def test_timer():
+    import ddm_amd
+    from ddm_amd.kernels import LaunchTimer
+    x, t = make(30, 50000, torch.bfloat16, 1)
+    timer = LaunchTimer()
+    ddm_amd.token_scores(x.cuda(), t.cuda(), top=3, timer=timer)
+    torch.cuda.synchronize()
+    assert 0.0 < timer.elapsed_ms() < 1000.0
+
+
+def test_tiny_and_huge_temperatures():
+    import ddm_amd
+    x, t = make(12, 3000, torch.float32, 4, special=False)
+    for temperature in (1e-3, 1e-30, 1e5, 1e30):
+        r = ddm_amd.token_scores(x.cuda(), t.cuda(), top=4, temperature=temperature)
+        check_scores(x, t, 4, temperature, r)

@@ -69,7 +69,7 @@ def test_entry_points_check_before_they_launch():
         x, dtype, n, v, ld, one, tb, temp, top, one, one, one, one, one, None, None, None, None, None, None)
     for kw, text in (({"dtype": 3}, "type"), ({"v": 0}, "columns"), ({"v": 1 << 20, "ld": 1 << 20}, "columns"),
                      ({"ld": 9}, "stride"), ({"n": -1}, "rows"), ({"n": 1 << 40}, "rows"), ({"tb": 2}, "targets"),
-                     ({"temp": 0.0}, "temperature"), ({"temp": float("inf")}, "temperature"), ({"top": 65}, "alternatives"),
+                     ({"temp": 0.0}, "temperature"), ({"temp": 1e-40}, "temperature"), ({"temp": float("inf")}, "temperature"), ({"top": 65}, "alternatives"),
                      ({"top": 2}, "null"), ({"x": None}, "null"), ({"v": 100000, "ld": 100000}, "null")):
         assert score(**kw) == _capi.DDM_E_ARG and text in last_error(), (kw, last_error())
     assert score(n=0) == 0
@@ -199,7 +199,7 @@ def test_gated_entry_points_check_before_they_launch():
                                 ({"lo": 9}, "stride"), ({"off": None}, "one sequence"), ({"s_out": None}, "null"),
                                 ({"s_in": one}, "one buffer"), ({"rows": 1 << 39, "d": 1 << 20, "g": 1 << 20, "ld": 1 << 20,
                                                                  "la": 1 << 20, "lo": 1 << 20}, "tiles"),
-                                ({"rows": 100000}, "scratch"))),
+                                ({"rows": 100000}, "scratch"), ({"ld": 1 << 23}, "row stride"))),
                         (grad, (({"h": None}, "null"), ({"ldh": 9}, "stride"), ({"lda": 4}, "stride"),
                                 ({"s0": None}, "null"), ({"ds": two}, "one buffer"))),
                         (step, (({"out": None}, "null"), ({"lo": 9}, "stride"), ({"d": 11}, "gates")))):
