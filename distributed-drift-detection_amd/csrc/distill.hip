@@ -367,7 +367,7 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
                     return rc;
             }
             with_part_shape(s, [&](auto nt, auto nv) {
-                k_distill<T, nt(), nv()><<<dim3((unsigned)(ceil_div(n, a.queues) * a.queues * s.parts)), nt(), 0, st>>>(a);
+                k_distill<T, nt(), nv()><<<dim3((unsigned)(a.tickets ? queue_grid(ceil_div(n, a.queues) * s.parts, a.queues) : n * s.parts)), nt(), 0, st>>>(a);
             });
             return launch_status("ddm_topk_distill");
         });

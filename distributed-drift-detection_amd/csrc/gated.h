@@ -149,7 +149,7 @@ __device__ __forceinline__ void with_scale(int scale, F f) {
 
 // ---- a tile's place -------------------------------------------------------------------------------
 struct Place {
-    int64_t tile;          // in the order of the recurrence
+    int64_t tile;          // in the order of the recurrence; from ntiles on: none
     int block;             // of channels
 };
 __device__ __forceinline__ Place take(const Args& a) {
@@ -252,11 +252,11 @@ __device__ __forceinline__ float carry_of_thread(const Args& a, int64_t tile, in
     // the tiles before in the group first: they run beside this one; the group before is what
     // there may be a wait for
     Step sum{1.0f, 0.0f};
-    for (int j = 0; j < in_group; j += 8) {
-        uint64_t w[8];
-        await<8>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
+    for (int j = 0; j < in_group; j += 4) {
+        uint64_t w[4];
+        await<4>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 4; ++i)
             if (j + i < in_group) sum = after(sum, Step{word_a(w[i]), word_b(w[i])});
     }
     const float carry = apply(sum, g > 0 ? word_a(await_one(a.inc + (g - 1) * a.dp + c)) : 0.0f);
@@ -331,14 +331,14 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
     const int col = waves ? wave : (int)threadIdx.x;
     if (col < cols) {
         Step all{1.0f, 0.0f};
-#pragma unroll
+#pragma unroll 2
         for (int w = 0; w < W; ++w) all = after(all, Step{l.a[w][col], l.b[w][col]});
         float carry = 0.0f;
         if (a.tickets) {
             const int64_t c = (int64_t)at.block * cols + col;
             carry = waves ? carry_of_wave(a, at.tile, c, all) : carry_of_thread(a, at.tile, c, all);
         }
-#pragma unroll
+#pragma unroll 2
         for (int w = 0; w < W; ++w) {
             const float next = apply(Step{l.a[w][col], l.b[w][col]}, carry);
             if (!waves || lane == 0) l.b[w][col] = carry;
@@ -471,7 +471,7 @@ inline int check(const char* who, int32_t dtype, int32_t gate_dtype, int64_t row
 
 // 0, or DDM_E_ARG where the grid has no room for the tiles, or a tile's rows lie too far apart for 32 bits.
 inline int check_tile(const char* who, const Shape& s, std::initializer_list<int64_t> ld_bytes) {
-    if (s.ntiles * s.ncb > INT32_MAX) {
+    if (s.ntiles * s.ncb > INT32_MAX - kQueues * kDies) {
         set_error("%s: %lld tiles of %d channel blocks", who, (long long)s.ntiles, s.ncb);
         return DDM_E_ARG;
     }
@@ -482,6 +482,10 @@ inline int check_tile(const char* who, const Shape& s, std::initializer_list<int
             return DDM_E_ARG;
         }
     return 0;
+}
+
+inline int64_t grid_of(const Args& a, const Shape& s) {
+    return a.tickets ? queue_grid(s.ntiles * (s.ncb / a.queues), a.queues) : s.ntiles * s.ncb;
 }
 
 inline int64_t scratch_bytes(const Shape& s, int64_t rows, int d) {

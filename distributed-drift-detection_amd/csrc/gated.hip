@@ -9,6 +9,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
     const Place at = take(a);
+    if (at.tile >= a.ntiles) return;
     const int cl = 1 << a.cl_bits, tg = threadIdx.x >> a.cl_bits, tr = (NT >> a.cl_bits) * R;
     const int c = (at.block * cl + (int)(threadIdx.x & (cl - 1))) * VEC;
     const int64_t row0 = at.tile * tr, r0 = row0 + tg * R;
@@ -228,7 +229,7 @@ extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const 
         if (int rc = begin(a, s, scratch, state_in, state_out, n * d, st)) return rc;
         if (rows == 0) return 0;
         const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
-        const dim3 grid((unsigned)(s.ntiles * s.ncb));
+        const dim3 grid((unsigned)grid_of(a, s));
         with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
             using X = decltype(xt);
             using L = decltype(lt);

@@ -11,6 +11,7 @@ __global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
     const Place at = take(a);
+    if (at.tile >= a.ntiles) return;
     const int cl = 1 << a.cl_bits, tg = (NT >> a.cl_bits) - 1 - (threadIdx.x >> a.cl_bits);
     const int tr = (NT >> a.cl_bits) * R;
     const int c = (at.block * cl + (int)(threadIdx.x & (cl - 1))) * VEC;
@@ -220,7 +221,7 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
         if (int rc = begin(a, s, scratch, d_state_out, d_state_in, n * d, st)) return rc;
         if (rows == 0) return 0;
         const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
-        const dim3 grid((unsigned)(s.ntiles * s.ncb));
+        const dim3 grid((unsigned)grid_of(a, s));
         const int64_t sums = ceil_div(rows * gates, 256);
         if (s.dl_parts && sums > INT32_MAX) {
             set_error("ddm_gated_scan_grad: %lld gate gradients", (long long)(rows * gates));

@@ -347,7 +347,7 @@ inline int check_rows(const char* who, int32_t dtype, int64_t n, int64_t v, int6
                       float temperature, int32_t top) {
     if (dtype != DDM_F32 && dtype != DDM_BF16 && dtype != DDM_F16) {
         set_error("%s: unknown type %d", who, (int)dtype);
-    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts - 8) {
+    } else if (n < 0 || v < 1 || v > kMaxColumns || ld < v || n > INT32_MAX / kMaxParts - 64) {
         set_error("%s: invalid argument (rows %lld, columns %lld of 1..%lld, row stride %lld)", who, (long long)n,
                   (long long)v, (long long)kMaxColumns, (long long)ld);
     } else if (target_bytes != 4 && target_bytes != 8) {
