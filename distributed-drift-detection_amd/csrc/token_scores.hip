@@ -399,6 +399,7 @@ __global__ __launch_bounds__(NT) void k_score_grad(GradArgs a) {
     float g_top = 0.0f;
     if (lane < a.top) {
         index = a.top_index[r * a.top + lane];
+        if (index >= a.v) index = -1;                  // the caller's, not read from this call
         if (index >= 0) g_top = a.d_top[r * a.top + lane];
     }
     float all_top = g_top;

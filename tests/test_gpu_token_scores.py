@@ -277,3 +277,18 @@ def test_tiny_and_huge_temperatures():
     for temperature in (1e-3, 1e-30, 1e5, 1e30):
         r = ddm_amd.token_scores(x.cuda(), t.cuda(), top=4, temperature=temperature)
         check_scores(x, t, 4, temperature, r)
+
+
+def test_alternatives_beyond_the_row_are_none():
+    import ddm_amd
+    x, t = make(13, 1000, torch.bfloat16, 5)
+    xc, tc = x.cuda(), t.cuda()
+    r = ddm_amd.token_scores(xc, tc, top=4)
+    d = torch.randn(13, 4, generator=torch.Generator().manual_seed(6)).cuda()
+    none, beyond = r.top_index.clone(), r.top_index.clone()
+    none[:, 1::2] = -1
+    beyond[:, 1] = 1000
+    beyond[:, 3] = 2**31 - 1
+    want = ddm_amd.token_scores_grad(xc, tc, r._replace(top_index=none), d_top=d)
+    got = ddm_amd.token_scores_grad(xc, tc, r._replace(top_index=beyond), d_top=d)
+    assert torch.equal(got, want)
