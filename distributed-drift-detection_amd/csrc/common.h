@@ -31,6 +31,13 @@ int timed(ddm_event_t begin, ddm_event_t end, hipStream_t s, F launch) {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// 0, or DDM_E_ARG where a launch has no room for the workgroups: under 2^32 work-items.
+inline int check_grid(const char* who, int64_t blocks, int threads) {
+    if (blocks < ((int64_t)1 << 32) / threads) return 0;
+    set_error("%s: %lld workgroups of %d (under 2^32 work-items a launch)", who, (long long)blocks, threads);
+    return DDM_E_ARG;
+}
+
 // A pointer into device (global) memory as the global address space: loads and stores
 // through it are global_* instructions.  A pointer loaded from a job table is generic, so
 // its accesses are flat_* instructions, which count on both vmcnt and lgkmcnt: every LDS

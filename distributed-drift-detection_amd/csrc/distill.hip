@@ -340,6 +340,7 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
     if (n == 0) return 0;
     const int size = dtype == DDM_F32 ? 4 : 2;
     const Shape s = distill_shape(n, vectors_of(logits, ld * size, v, 16 / size));
+    if (int rc = check_grid("ddm_topk_distill", n * s.parts + kQueues * kDies * s.parts, s.nt)) return rc;
     if (!logits || !loss || (k && (!index || !logprob)) || (grad && grad_ld < v) || (s.parts > 1 && !scratch)) {
         set_error("ddm_topk_distill: invalid argument (null pointer or gradient stride)");
         return DDM_E_ARG;

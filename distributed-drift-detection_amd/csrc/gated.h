@@ -471,8 +471,8 @@ inline int check(const char* who, int32_t dtype, int32_t gate_dtype, int64_t row
 
 // 0, or DDM_E_ARG where the grid has no room for the tiles, or a tile's rows lie too far apart for 32 bits.
 inline int check_tile(const char* who, const Shape& s, std::initializer_list<int64_t> ld_bytes) {
-    if (s.ntiles * s.ncb > INT32_MAX - kQueues * kDies) {
-        set_error("%s: %lld tiles of %d channel blocks", who, (long long)s.ntiles, s.ncb);
+    if (check_grid(who, s.ntiles * s.ncb + kQueues * kDies, NT)) {
+        set_error("%s: %lld tiles of %d channel blocks (under 2^32 work-items a launch)", who, (long long)s.ntiles, s.ncb);
         return DDM_E_ARG;
     }
     const int64_t rows = (int64_t)(NT >> s.cl_bits) * s.r;

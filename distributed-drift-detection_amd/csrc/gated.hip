@@ -253,12 +253,16 @@ extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const 
         return DDM_E_ARG;
     }
     const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype);
-    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
-    const int64_t blocks = ceil_div(rows * (d / vec), 256);
-    if (blocks > INT32_MAX) {
-        set_error("ddm_gated_step: %lld rows of %lld channels", (long long)rows, (long long)d);
+    auto in_state_out = [&](const void* p, int64_t bytes) {      // a row of it is read after another is written
+        return (uintptr_t)p < (uintptr_t)(state_out + rows * d) && (uintptr_t)state_out < (uintptr_t)p + bytes;
+    };
+    if (in_state_out(x, ((rows - 1) * ld_x + d) * es) || in_state_out(log_a, ((rows - 1) * ld_a + gates) * gs)) {
+        set_error("ddm_gated_step: the state after overlaps the inputs");
         return DDM_E_ARG;
     }
+    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
+    const int64_t blocks = ceil_div(rows * (d / vec), 256);
+    if (int rc = check_grid("ddm_gated_step", blocks, 256)) return rc;
     const hipStream_t st = as_hip(stream);
     return timed(ev_begin, ev_end, st, [&] {
         Args a{};

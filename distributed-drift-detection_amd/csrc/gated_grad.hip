@@ -189,6 +189,8 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
     if (int rc = check_tile("ddm_gated_scan_grad", s,
                             {ld_x * es, ld_a * gs, ld_h * es, ld_dh * es, ld_dx * es, ld_da * gs}))
         return rc;
+    const int64_t sums = s.dl_parts ? ceil_div(rows * gates, 256) : 0;
+    if (int rc = check_grid("ddm_gated_scan_grad", sums, 256)) return rc;
     if (scratch_bytes(s, rows, (int)d) && !scratch) {
         set_error("ddm_gated_scan_grad: invalid argument (no scratch)");
         return DDM_E_ARG;
@@ -222,11 +224,6 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
         if (rows == 0) return 0;
         const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
         const dim3 grid((unsigned)grid_of(a, s));
-        const int64_t sums = ceil_div(rows * gates, 256);
-        if (s.dl_parts && sums > INT32_MAX) {
-            set_error("ddm_gated_scan_grad: %lld gate gradients", (long long)(rows * gates));
-            return DDM_E_ARG;
-        }
         int rc = 0;
         with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
             using X = decltype(xt);
@@ -236,7 +233,7 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
             else
                 k_gated_grad<X, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
             rc = launch_status("ddm_gated_scan_grad");
-            if (!rc && s.dl_parts) k_gated_sum<L><<<dim3((unsigned)sums), 256, 0, st>>>(a, gates, s.dl_parts);
+            if (!rc && sums) k_gated_sum<L><<<dim3((unsigned)sums), 256, 0, st>>>(a, gates, s.dl_parts);
         });
         return rc ? rc : launch_status("ddm_gated_scan_grad");
     });

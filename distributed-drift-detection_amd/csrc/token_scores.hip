@@ -481,6 +481,7 @@ extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, in
     if (n == 0) return 0;
     const int size = dtype == DDM_F32 ? 4 : 2;
     const Shape s = shape_of(n, vectors_of(logits, ld * size, v, 16 / size), true);
+    if (int rc = check_grid("ddm_token_scores", n * s.parts, s.nt)) return rc;
     if (!logits || !target || !logprob || !entropy || !stats || !rank || !err || (top && (!top_logprob || !top_index)) ||
         (s.parts > 1 && !scratch)) {
         set_error("ddm_token_scores: invalid argument (null pointer)");
@@ -526,6 +527,7 @@ extern "C" int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t 
     }
     const int size = dtype == DDM_F32 ? 4 : 2;
     const Shape s = shape_of(n, vectors_of(logits, ld * size, v, 16 / size), false);
+    if (int rc = check_grid("ddm_token_scores_grad", n * s.parts, s.nt)) return rc;
     const hipStream_t st = as_hip(stream);
     return timed(ev_begin, ev_end, st, [&] {
         return with_type(dtype, [&](auto type) {

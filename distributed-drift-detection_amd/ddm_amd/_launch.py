@@ -91,6 +91,8 @@ def dense(t):
 
 
 def _span(t):
+    if t.is_contiguous():
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 

@@ -75,8 +75,8 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
         if out.shape != x.shape or out.dtype != x.dtype:
             raise ValueError(f"out must be {x.dtype} {list(x.shape)}, got {out.dtype} {list(out.shape)}")
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-        for t in (x, log_a):
-            if overlap(out, t) and not (t is x and same):
+        for t in (x, log_a, offsets, state):
+            if t is not None and overlap(out, t) and not (t is x and same):
                 raise ValueError("out overlaps an input without being x")
     else:
         ld_out = d

@@ -42,7 +42,7 @@ def _logits(logits):
     return n, v, ld
 
 
-def _check_out(out, logits):
+def _check_out(out, logits, *others):
     if out is None:
         return
     rows_of("out", out)
@@ -51,6 +51,8 @@ def _check_out(out, logits):
     same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
     if not same and overlap(out, logits):
         raise ValueError("out overlaps the logits without being them")
+    if any(t is not None and overlap(out, t) for t in others):
+        raise ValueError("out overlaps another argument")
 
 
 def _new_like(out, logits):
@@ -94,7 +96,7 @@ def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d
     """Gradient by the logits of  d_logprob . logprob + d_entropy . entropy + d_top . top_logprob
     (float32 [n], [n], [n, top]; None: zero), in the logits' type.  `scores` is what
     token_scores returned for the same logits and targets.  out: None, the logits themselves
-    (overwritten), or a tensor of their shape apart from them."""
+    (overwritten), or a tensor of their shape apart from every argument."""
     n, v, ld = _logits(logits)
     shaped("targets", targets, (n,), torch.int32, torch.int64)
     shaped("scores.stats", scores.stats, (n, 2), torch.float32)
@@ -109,7 +111,7 @@ def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d
         index, top = scores.top_index, scores.top_index.shape[1]
         shaped("scores.top_index", index, (n, top), torch.int32)
         shaped("d_top", d_top, (n, top), torch.float32)
-    _check_out(out, logits)
+    _check_out(out, logits, targets, scores.stats, scores.entropy, index, d_logprob, d_entropy, d_top)
     given = (logits, targets, scores.stats, scores.entropy, index, d_logprob, d_entropy, d_top, out)
     context, s = launch_on(logits, stream, given)
     with context:
@@ -151,7 +153,7 @@ def topk_distill(logits, index, logprob, tail="rest", temperature=1.0, weight=No
     shaped("logprob", logprob, (n, k), torch.float32)
     if weight is not None:
         shaped("weight", weight, (n,), torch.float32)
-    _check_out(out, logits)
+    _check_out(out, logits, index, logprob, weight)
     code = DTYPES[logits.dtype]
     context, s = launch_on(logits, stream, (logits, index, logprob, weight, out))
     with context:

@@ -207,3 +207,38 @@ def test_gated_entry_points_check_before_they_launch():
             assert call(**kw) == _capi.DDM_E_ARG and text in last_error(), (kw, last_error())
     assert lib.ddm_gated_scan_scratch_bytes(0, 8, 8, 0, 0) == 0
     assert lib.ddm_gated_scan_scratch_bytes(100000, 8, 8, 0, 0) > 0
+
+
+def test_results_over_other_arguments():
+    base = torch.zeros(44)
+    out = base[:40].view(4, 10)
+    for kw in ({"d_logprob": base[39:43]}, {"d_entropy": base[:4]}):
+        with pytest.raises(ValueError, match="overlaps another"):
+            tokens.token_scores_grad(X, T, scores(), out=out, **kw)
+    index = torch.zeros(4, 1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="overlaps another"):
+        tokens.topk_distill(X, index, base[38:42].view(4, 1), out=out)
+    with pytest.raises(ValueError, match="overlaps another"):
+        tokens.topk_distill(X, index, torch.zeros(4, 1), weight=base[::11], out=out)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        gated.gated_scan(X, G, state=base[20:30].view(1, 10), out=out)
+    x, log_a = 1 << 20, 1 << 21         # 4 rows of 10 and of 5 float32: 160 and 80 bytes
+    for state in (x + 156, x - 156, log_a + 76, log_a - 156):
+        rc = _capi.lib.ddm_gated_step(x, 0, 10, log_a, 0, 5, 4, 10, 5, 0, None, state, 1 << 22, 10, None, None, None)
+        assert rc == _capi.DDM_E_ARG and "overlaps" in last_error(), last_error()
+
+
+def test_launches_have_room():
+    one, two, lib = ctypes.c_void_p(256), ctypes.c_void_p(512), _capi.lib
+    n = (1 << 24) + 5                   # rows of 4100 bfloat16: a workgroup of 256 each
+    for rc in (lib.ddm_token_scores(one, 1, n, 4100, 4100, one, 8, 1.0, 0, one, one, one, one, one, None, None, one, None,
+                                    None, None),
+               lib.ddm_token_scores_grad(one, 1, n, 4100, 4100, one, 8, 1.0, 0, one, one, None, None, None, None, one,
+                                         4100, None, None, None),
+               lib.ddm_topk_distill(one, 1, n, 4100, 4100, one, 8, one, 1, 0, 1.0, None, one, one, 4100, one, None, None,
+                                    None),
+               lib.ddm_gated_step(one, 0, 1 << 20, one, 0, 1, 4096, 1 << 20, 1, 0, None, two, one, 1 << 20, None, None,
+                                  None),
+               lib.ddm_gated_scan_grad(one, 1, 2049, one, 1, 3, one, 2049, one, 2049, (1 << 32) // 3 + 1, 2049, 3, one, 2,
+                                       0, None, None, two, one, 2049, one, 3, 1, one, None, None, None)):
+        assert rc == _capi.DDM_E_ARG and "work-items" in last_error(), last_error()
