@@ -14,6 +14,8 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     const int c = (at.block * cl + (int)(threadIdx.x & (cl - 1))) * VEC;
     const int64_t row0 = at.tile * tr, r0 = row0 + tg * R;
     const bool active = c < a.d;
+    Sequences seq{};
+    if (a.off) seq = find_sequences(a, row0);
     Raw<X, VEC> x[R];
     Gates<L, VEC, OWN> l[R];
     const uint32_t lane_x = tg * R * (uint32_t)a.ld_x + c * (uint32_t)sizeof(typename X::E);
@@ -39,11 +41,10 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     const Marks m(marks, tr);
     uint32_t begins, ends, inside;
     if (a.off) {
-        mark_rows(a, row0, tr, m);
+        mark_rows(a, row0, tr, m, seq);
         begins = Marks::lane<R>(m.begin_bits, tg * R);
         ends = Marks::lane<R>(m.end_bits, tg * R);
-        const int64_t end = a.off[a.n];
-        inside = rows_within<R>(r0, a.off[0], end < a.rows ? end : a.rows);
+        inside = rows_within<R>(r0, seq.first, seq.end);
     } else {
         begins = r0 == 0;
         ends = a.rows - 1 >= r0 && a.rows - 1 < r0 + R ? 1u << (int)(a.rows - 1 - r0) : 0u;
