@@ -7,8 +7,9 @@
 // into tiles; a workgroup holds one tile of rows and channels in registers, reduces it to
 // its (A, B), gets the state before it from the tiles before it, and runs the recurrence from
 // there: x and l are read once and h is written once, which is the floor.  The state comes
-// by a look-back of fixed shape: tiles form groups, a tile reads the (A, B) of those before it in
-// its group and the state after the group before, which that group's last tile publishes.
+// by a look-back of fixed shape: tiles form groups and groups form rows of groups; a tile reads the
+// (A, B) of those before it in its group, of the groups before that one in its row, which a group's
+// last tile publishes, and the state after the row before.
 // What is composed in which order depends on the sizes alone, so results do not change from
 // run to run.  Tiles are taken in order by a ticket, so that a tile only ever waits for tiles
 // that already run.  A published word is one 8-byte store that carries its own validity (unset
@@ -81,10 +82,10 @@ struct Args {
     int64_t n;
     const float *state_in, *dstate;      // may be NULL (0)
     float* state_out;                     // state after, or gradient of the state before
-    int cl_bits, ncb, group;             // lanes across channels (log2), channel blocks, tiles a group
+    int cl_bits, ncb, group;             // lanes across channels (log2), channel blocks, tiles a group and groups a row
     int64_t ntiles;
     uint32_t *tickets, queues;            // NULL: one tile, no chain
-    uint64_t *agg, *inc, *far;            // [ntiles][dp], [groups][dp], [groups / 64][dp]
+    uint64_t *agg, *inc, *far;            // [ntiles][dp], [groups][dp], [rows of groups][dp]
     int64_t dp;
     float* dl_part;                       // [rows][parts a row] or NULL: dl itself
     int dl_width;                         // lanes summed within a wave
@@ -176,7 +177,7 @@ struct Marks {
     }
 };
 // The sequences that may begin or end in a tile, one a thread, asked for before the tile's rows are, so
-// that nobody waits for them behind those (65536 x 2048 in 37 sequences: 242 -> NEW us).
+// that nobody waits for them behind those (65536 x 2048 in 37 sequences: 242 -> 220 us).
 struct Sequences {
     int64_t s, b, e, first, end;       // a thread's first one; where the first begins and the last ends
 };
@@ -259,31 +260,39 @@ __device__ __forceinline__ uint64_t await_one(const uint64_t* p) {
     return w[0];
 }
 
-// The state before a tile, for one channel a thread, given the tile's own step.  Tiles form groups of
-// a.group; the last of a group publishes the state after it.
-__device__ __forceinline__ float carry_of_thread(const Args& a, int64_t tile, int64_t c, const Step& all) {
-    const int64_t g = tile / a.group;
-    const int in_group = (int)(tile % a.group);
-    const bool last = in_group == a.group - 1, more = tile + 1 < a.ntiles;
-    if (!last && more) publish(a.agg + tile * a.dp + c, word(all.a, all.b));
-    // the tiles before in the group first: they run beside this one; the group before is what
-    // there may be a wait for
-    Step sum{1.0f, 0.0f};
-    for (int j = 0; j < in_group; j += 4) {
+// The state before a tile, for one channel a thread, given the tile's own step.  a.group (8) tiles form
+// a group, whose last one publishes the group's step; as many groups form a row, and the state after
+// those is passed on one by one.  (Groups of 16 that pass the state on themselves: 1000003 x 32 bf16
+// 95 us, now 71; 200000 x 17 f32 with the gradient 101, now 80.  Rows of 16 groups of 16: 77 and 85.)
+__device__ __forceinline__ Step thread_steps(const uint64_t* p, int64_t stride, int count) {
+    Step s{1.0f, 0.0f};
+    for (int j = 0; j < count; j += 4) {
         uint64_t w[4];
-        await<4>(a.agg + (g * a.group + j) * a.dp + c, a.dp, in_group - j, w);
+        await<4>(p + j * stride, stride, count - j, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (j + i < in_group) sum = after(sum, Step{word_a(w[i]), word_b(w[i])});
+            if (j + i < count) s = after(s, Step{word_a(w[i]), word_b(w[i])});
     }
-    const float carry = apply(sum, g > 0 ? word_a(await_one(a.inc + (g - 1) * a.dp + c)) : 0.0f);
-    if (last && more) publish(a.inc + g * a.dp + c, word(apply(all, carry), 0.0f));
+    return s;
+}
+__device__ __forceinline__ float carry_of_thread(const Args& a, int64_t tile, int64_t c, const Step& all) {
+    const int64_t g = tile / a.group, h = g / a.group;
+    const int in_group = (int)(tile % a.group), in_groups = (int)(g % a.group);
+    const bool last = in_group == a.group - 1, more = tile + 1 < a.ntiles;
+    if (!last && more) publish(a.agg + tile * a.dp + c, word(all.a, all.b));
+    const Step tiles = thread_steps(a.agg + g * a.group * a.dp + c, a.dp, in_group);
+    if (last && more) {
+        const Step group = after(tiles, all);
+        publish(a.inc + g * a.dp + c, word(group.a, group.b));
+    }
+    const Step groups = thread_steps(a.inc + h * a.group * a.dp + c, a.dp, in_groups);
+    const float carry = apply(tiles, apply(groups, h > 0 ? word_a(await_one(a.far + (h - 1) * a.dp + c)) : 0.0f));
+    if (last && in_groups == a.group - 1 && more) publish(a.far + h * a.dp + c, word(apply(all, carry), 0.0f));
     return carry;
 }
 
 // The same for one channel a wave, where there are few: a lane for each tile before in the group, then
-// a lane for each group before (its step, published by its last tile), so nothing passes from group to
-// group one by one.  Every 64 groups the state itself is passed on.
+// a lane for each group before; groups and rows are of 64.
 __device__ __forceinline__ Step wave_steps(const uint64_t* p, int64_t stride, int count) {
     const int lane = threadIdx.x & 63;
     Step s{1.0f, 0.0f};
@@ -402,7 +411,7 @@ struct Gates {
 struct Shape {
     int vec, cl_bits, ncb, r, group, dl_width, dl_parts;
     int64_t ntiles, dp;
-    int64_t words() const { return ntiles > 1 ? (ntiles + groups() + ceil_div(groups(), 64)) * dp : 0; }
+    int64_t words() const { return ntiles > 1 ? (ntiles + groups() + ceil_div(groups(), group)) * dp : 0; }
     int64_t groups() const { return ceil_div(ntiles, group); }
 };
 inline Shape shape_of(int64_t rows, int d, int share, int vec, bool grad) {
@@ -418,7 +427,7 @@ inline Shape shape_of(int64_t rows, int d, int share, int vec, bool grad) {
     s.r = grad ? 8 : 16;                              // four operands a row, not two
     if (ceil_div(rows, tg * s.r) * s.ncb < 256 || tg * s.r > 4096) s.r = 4;
     s.ntiles = ceil_div(rows, (int64_t)tg * s.r);
-    s.group = s.cl_bits == 6 ? 16 : 64;              // what a tile reads of others stays under a tenth of its own
+    s.group = (vec << s.cl_bits) > W ? 8 : 64;       // a thread's words in turn, a wave's at once
     s.dp = (int64_t)(s.ncb << s.cl_bits) * vec;
     s.dl_width = 1;
     s.dl_parts = 0;
