@@ -17,8 +17,9 @@
 // is written from there: every logit is read once, and with 6 workgroups on a CU the others load or
 // store while one waits.  The row's first part finishes it: it alone looks up the student's logits at
 // the teacher's columns (64 lines a row) and writes the gradient there, so the other parts leave
-// those columns out.  (A whole row in the registers of 1024 lanes leaves one workgroup a CU and
-// nothing to do while it sums; reading twice costs half again the traffic.)
+// those columns out.  4096 x 131072 bf16 with 64 alternatives: 435 us, 4.9 TB/s, what a copy reaches.
+// (A whole row in the registers of 1024 lanes leaves one workgroup a CU and nothing to do while
+// it sums, 549 us; reading twice costs half again the traffic, 570 us.)
 #include "logits.h"
 #include "words.h"
 
@@ -38,7 +39,7 @@ struct DistillArgs {
     char* out;                 // NULL: the loss alone
     uint32_t *tickets, queues; // one part a row: NULL
     uint64_t* words;           // [n][parts + 2]: m, s of a part's columns that are not kept (renorm: of
-                               // all); then the row's Bulk
+                               // all); then the row's Bulk.  The loss alone: [n][parts], no Bulk
 };
 
 // The teacher's alternatives of a row, one a lane of a wave.
@@ -262,7 +263,8 @@ __global__ __launch_bounds__(NT) void k_distill(DistillArgs a) {
 
 // ---- the loss alone -----------------------------------------------------------------------------------
 // Nothing is to be written after the sums, so no part waits: a launch for the parts and one, a wave a
-// row, that joins them.
+// row, that joins them.  1777 x 50021 float16: 39 + 5 us, 4.0 TB/s in all, the vector unit as busy as
+// the memory (with parts that wait 60 us).
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) void k_distill_parts(DistillArgs a) {
     __shared__ uint32_t bits[NT * NV / 4];

@@ -4,6 +4,10 @@
 namespace ddm {
 namespace gated {
 
+// A tile's steps stay in registers, two float32 an entry; 16 rows a lane let two workgroups share a CU.
+// 65536 x 2048 bf16, "unit", 37 sequences: 228 us, 3.5 TB/s; one sequence of them 207.  What is above
+// the 165 us of the same kernel without the chain is tiles waiting for tiles.  (With the steps computed
+// again after the wait, three workgroups fit a CU: "unit" 235 us, "none" no faster.)
 template <typename X, typename L, int VEC, bool OWN, int R>
 __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     extern __shared__ int32_t marks[];
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     }
 }
 
-// One row a sequence: elementwise, the state's row beside it.
+// One row a sequence: elementwise, the state's row beside it.  256 x 2048 bf16: 3.6 us, a launch's time.
 template <typename X, typename L, int VEC, bool OWN>
 __global__ __launch_bounds__(256) void k_gated_step(Args a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

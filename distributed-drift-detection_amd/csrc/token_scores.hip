@@ -4,13 +4,16 @@
 //
 // With d_i = (x_i - m) / T, m near the row's maximum, S = sum e^d_i, U = sum e^d_i d_i:
 //   log p_i = d_i - log S,   H = log S - U / S,   rank = #{x_i > x_t or x_i = x_t, i < t}.
-// The pass is bound by reading the logits; what it computes per entry (about 13 vector
-// operations, one of them an exponential at a quarter of the rate) is just under what hides
-// behind that for 16-bit logits.  A row is cut into parts of at most kPartBytes, one a
-// workgroup, so that several workgroups share a CU and one's sums run behind another's loads;
-// few rows are cut finer, until there are enough workgroups for the chip.  Parts meet in a
-// second small launch.  No atomic decides an order: every sum is a fixed tree, and the
-// alternatives are ordered by (value, index).
+// The pass is bound by reading the logits; what it computes per entry (12 vector instructions with
+// the alternatives, one of them an exponential at a quarter of the rate) takes as long as that
+// for 16-bit logits.  A row is cut into parts (shape_of), one a workgroup, so that several workgroups
+// share a CU and one's sums run behind another's loads; few rows are cut finer, until there are
+// enough workgroups for the chip.  Parts meet in a second small launch.  No atomic decides an
+// order: every sum is a fixed tree, and the alternatives are ordered by (value, index).
+// Measured: 8192 x 131072 bf16 with 32 alternatives 415 us, 5.2 TB/s and the vector unit busy all the
+// time; 4096 x 65536 bf16 without 150 us; 1000 x 50021 float32 with 5 50 us, 4.0 TB/s; one row of
+// 131072 bf16 with 20 in 8 + 6.5 us, latencies of the two launches.  (A copy of 2 GB runs at
+// 4.9 TB/s, reads and writes together.)
 #include "logits.h"
 
 namespace ddm {
@@ -365,7 +368,8 @@ __global__ __launch_bounds__(NT) void k_score_join(ScoreArgs a) {
 // dx_i = (-p_i (A + B log p_i) + [i = t] g_lp + [i = index_k] g_top,k) / T with
 // A = g_lp + sum g_top + g_H H, B = g_H: elementwise from the forward's statistics, reading and
 // writing every logit once.  The few columns with a term of their own are written again after
-// the rest of their part, in full, by one lane each.
+// the rest of their part, in full, by one lane each.  Bound by that traffic: 4096 x 65536 bf16 in
+// 176 us, 6.1 TB/s, the logits partly still in the last cache from the forward.
 struct GradArgs {
     const char* x;
     int64_t n, v, ld_bytes, out_ld_bytes;

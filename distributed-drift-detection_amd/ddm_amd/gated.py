@@ -124,7 +124,8 @@ def gated_scan_grad(x, log_a, h, d_h, offsets=None, state=None, d_state=None, sc
 
 def gated_step(x, log_a, state=None, scale="none", out_state=None, stream=None, timer=None):
     """One row of every sequence: row s of x [n, d] and log_a [n, gates] continues state[s] (float32,
-    None: 0).  Returns (h in x's type, the state after); out_state may be `state` itself."""
+    None: 0).  Returns (h in x's type, the state after); out_state may be `state` itself, and lies apart
+    from x and log_a."""
     rows, d, gates, ld_x, ld_a = _inputs(x, log_a)
     mode = _scale(scale)
     for name, t in (("state", state), ("out_state", out_state)):

@@ -764,8 +764,8 @@ int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, int64_t v, in
                      void* scratch, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
 /* Gradient of sum d_logprob logprob + d_entropy entropy + d_top top_logprob by the logits, in
  * their type, to out (row stride out_ld): the logits' own buffer with their stride, or one
- * that does not overlap it.  stats, entropy and top_index are the forward's;
- * d_logprob and d_entropy may be NULL (0), top 0 leaves the alternatives out. */
+ * that does not overlap it.  stats, entropy and top_index are the forward's (an index outside [0, v)
+ * is none); d_logprob and d_entropy may be NULL (0), top 0 leaves the alternatives out. */
 int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t n, int64_t v, int64_t ld, const void* target,
                           int32_t target_bytes, float temperature, int32_t top, const float* stats,
                           const float* entropy, const int32_t* top_index, const float* d_logprob,
@@ -821,7 +821,8 @@ int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, const void* 
                         const float* d_state_out, float* d_state_in, void* d_x, int64_t ld_dx, void* d_log_a,
                         int64_t ld_da, int32_t fill, void* scratch, ddm_stream_t stream, ddm_event_t ev_begin,
                         ddm_event_t ev_end);
-/* One row a sequence (row s continues state s); state_out may be state_in. */
+/* One row a sequence (row s continues state s); state_out may be state_in, and overlaps neither x
+ * nor log_a. */
 int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const void* log_a, int32_t gate_dtype, int64_t ld_a,
                    int64_t rows, int64_t d, int64_t gates, int32_t scale, const float* state_in, float* state_out,
                    void* out, int64_t ld_out, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
