@@ -80,6 +80,14 @@ def test_a_long_stream():
     check(*make(40001, 2, 1, F, F, 4, 2), "ewma", True)
 
 
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("rows,d,g,seqs", [(3000, 40, 40, 513), (5000, 3, 1, 5000), (900, 64, 64, 9000), (20, 70, 7, 2000),
+                                           (40001, 12, 12, 600)])
+def test_many_sequences(dtype, rows, d, g, seqs):
+    """More sequences than a workgroup has threads, most of them empty or of a row; narrow rows of many tiles."""
+    check(*make(rows, d, g, dtype, dtype, 7, seqs), "ewma", True)
+
+
 def test_the_same_every_time():
     import ddm_amd
     x, lam, off, state = on(*make(20000, 512, 512, B, B, 5, 6))
