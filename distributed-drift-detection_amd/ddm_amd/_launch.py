@@ -99,4 +99,11 @@ def _span(t):
 
 def overlap(a, b):
     (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    if not (a0 < b1 and b0 < a1):
+        return False
+    if a.dim() == 2 and b.dim() == 2 and a.stride(1) == 1 and b.stride(1) == 1:
+        row = a.stride(0) * a.element_size()
+        if row > 0 and row == b.stride(0) * b.element_size():       # columns of one buffer
+            apart, wide_a, wide_b = (b0 - a0) % row, a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+            return apart < wide_a or apart + wide_b > row
+    return True

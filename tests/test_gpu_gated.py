@@ -128,6 +128,20 @@ def test_strides(dtype, shift, pad):
     assert torch.equal(same[a:b], h[a:b]) and torch.equal(after2, after)
 
 
+@pytest.mark.parametrize("dtype,d,g", [(F, 40, 40), (B, 64, 64), (B, 30, 6)])
+def test_inputs_and_gates_in_one_buffer(dtype, d, g):
+    """As a projection gives them; the result over the inputs, the gates as they were."""
+    import ddm_amd
+    x, lam, off, state = make(2500, d, g, dtype, dtype, 11, 5)
+    both = torch.cat([x, lam], 1).cuda()
+    h, after = ddm_amd.gated_scan(both[:, :d], both[:, d:], off.cuda(), state.cuda(), scale="unit", out=both[:, :d])
+    ref = gated64(x, lam, off, state, "unit")
+    a, b = int(off[0]), int(off[-1])
+    close(h[a:b], *(t[a:b] for t in ref["h"]), dtype)
+    close(after, *ref["state"])
+    assert torch.equal(both[:, d:].cpu(), lam) and torch.equal(both[:a, :d].cpu(), x[:a])
+
+
 def test_one_row_of_gates_for_all_rows():
     import ddm_amd
     x, lam, off, state = make(900, 96, 12, F, F, 8, 4)

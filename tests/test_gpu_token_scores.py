@@ -292,3 +292,20 @@ def test_alternatives_beyond_the_row_are_none():
     want = ddm_amd.token_scores_grad(xc, tc, r._replace(top_index=none), d_top=d)
     got = ddm_amd.token_scores_grad(xc, tc, r._replace(top_index=beyond), d_top=d)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(13, 517), (12, 9001)])
+def test_gradient_beside_the_logits(dtype, n, v):
+    """Two halves of one buffer; the logits stay as they were."""
+    import ddm_amd
+    x, t = make(n, v, dtype, 9)
+    both = torch.zeros(n, 2 * v, dtype=dtype, device="cuda")
+    both[:, :v] = x.cuda()
+    r = ddm_amd.token_scores(both[:, :v], t.cuda())
+    d = torch.randn(n, generator=torch.Generator().manual_seed(1)).cuda()
+    want = ddm_amd.token_scores_grad(x.cuda(), t.cuda(), r, d_logprob=d)
+    got = ddm_amd.token_scores_grad(both[:, :v], t.cuda(), r, d_logprob=d, out=both[:, v:])
+    # the same numbers; a product that is -0 may come as +0, by the instruction that rounds it to float16
+    assert ((got == want) | (got.isnan() & want.isnan())).all()
+    assert torch.equal(both[:, :v].cpu().view(torch.uint8), x.view(torch.uint8))

@@ -242,3 +242,20 @@ def test_launches_have_room():
                lib.ddm_gated_scan_grad(one, 1, 2049, one, 1, 3, one, 2049, one, 2049, (1 << 32) // 3 + 1, 2049, 3, one, 2,
                                        0, None, None, two, one, 2049, one, 3, 1, one, None, None, None)):
         assert rc == _capi.DDM_E_ARG and "work-items" in last_error(), last_error()
+
+
+def test_columns_of_one_buffer_lie_apart():
+    from ddm_amd._launch import overlap
+    base = torch.zeros(6, 30)
+    cut = lambda a, b, r=slice(0, 6): base[r, a:b]  # noqa: E731
+    for a, b, want in ((cut(0, 10), cut(10, 25), False), (cut(0, 10), cut(9, 25), True), (cut(10, 25), cut(0, 10), False),
+                       (cut(10, 25), cut(0, 11), True), (cut(20, 30), cut(0, 20, slice(1, 6)), False),
+                       (cut(0, 10, slice(0, 3)), cut(0, 10, slice(3, 6)), False), (cut(0, 10), cut(0, 10), True),
+                       (cut(0, 10, slice(0, 4)), cut(5, 8, slice(2, 6)), True), (cut(0, 30), cut(29, 30), True),
+                       (base.view(12, 15)[:, :5], cut(5, 15), True), (base[0], cut(3, 5), True)):
+        assert overlap(a, b) == want and overlap(b, a) == want, (a.shape, b.shape, want)
+    # a projection's inputs and gates side by side, the result over the inputs
+    with pytest.raises(ValueError, match="on the GPU"):
+        gated.gated_scan(cut(0, 20), cut(20, 30), out=cut(0, 20))
+    with pytest.raises(ValueError, match="on the GPU"):
+        tokens.token_scores_grad(cut(0, 10, slice(0, 4)), T, scores(), out=cut(10, 20, slice(0, 4)))
