@@ -312,7 +312,8 @@ __device__ __forceinline__ int64_t target_at(const void* t, int wide, int64_t i)
 }
 
 constexpr int kMaxTop = 64;              // alternatives of a row: one a lane
-constexpr int kMaxParts = 64;            // parts of a row, as well
+constexpr int kMaxParts = 64;            // parts that a short list of rows is cut into, as well; the longest
+                                         // float32 row that does not start aligned takes 65
 constexpr int64_t kMaxColumns = 1 << 19;
 
 struct Shape {

@@ -336,10 +336,10 @@ __global__ __launch_bounds__(NT) void k_score_join(ScoreArgs a) {
     const float c = kLog2e / a.temperature;
     Part p = no_part();
     uint32_t ahead = 0;
-    if (lane < a.parts) {                              // every wave for itself
-        const float4 q = a.part_sum[r * a.parts + lane];
-        p = Part{q.x, q.y, q.z};
-        ahead = __float_as_uint(q.w);
+    for (int i = lane; i < a.parts; i += 64) {         // every wave for itself
+        const float4 q = a.part_sum[r * a.parts + i];
+        p = merge(p, Part{q.x, q.y, q.z}, c);
+        ahead += __float_as_uint(q.w);
     }
     p = wave_merge(p, c);
 #pragma unroll

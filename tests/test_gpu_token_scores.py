@@ -309,3 +309,24 @@ def test_gradient_beside_the_logits(dtype, n, v):
     # the same numbers; a product that is -0 may come as +0, by the instruction that rounds it to float16
     assert ((got == want) | (got.isnan() & want.isnan())).all()
     assert torch.equal(both[:, :v].cpu().view(torch.uint8), x.view(torch.uint8))
+
+
+@pytest.mark.parametrize("v,shift", [(524285, 0), (524286, 0), (524287, 0), (524288, 0), (524288, 1), (524286, 3), (524287, 2)])
+@pytest.mark.parametrize("top", [0, 20])
+def test_the_longest_rows_to_their_end(v, shift, top):
+    """Float32 rows of most columns, aligned or not: what counts lies in their last three columns."""
+    import ddm_amd
+    n = 3
+    g = torch.Generator().manual_seed(v + shift)
+    x = torch.randn(n, v, generator=g)
+    x[:, -3:] += torch.tensor([12.0, 14.0, 13.0])
+    x[1, -1] = 20.0
+    t = torch.tensor([v - 1, v - 2, v - 3])
+    flat = torch.zeros(shift + n * v, device="cuda")
+    view = flat[shift:].view(n, v)
+    view.copy_(x)
+    r = ddm_amd.token_scores(view, t.cuda(), top=top)
+    ref = check_scores(x, t, top, 1.0, r)
+    d = torch.randn(n, generator=g)
+    want, tol = scores_grad64(x, t, ref, 1.0, d_logprob=d, d_entropy=d)
+    close(ddm_amd.token_scores_grad(view, t.cuda(), r, d_logprob=d.cuda(), d_entropy=d.cuda()), want, tol)
