@@ -227,10 +227,9 @@ __global__ __launch_bounds__(NT) void k_distill(DistillArgs a) {
     if (finish) {
         if (a.tickets) {
             p = no_part();
-            if ((int)threadIdx.x < a.parts) {
-                const uint64_t w = wait_for(words + threadIdx.x);
-                p.m = word_a(w);
-                p.s = word_b(w);
+            for (int i = threadIdx.x; i < a.parts; i += 64) {
+                const uint64_t w = wait_for(words + i);
+                p = merge(p, Part{word_a(w), word_b(w), 0.0f}, c);
             }
             p = wave_merge(p, c);
         }
@@ -287,14 +286,14 @@ __global__ __launch_bounds__(64) void k_distill_join(DistillArgs a) {
     const int64_t r = blockIdx.x;
     const Row<T> row(a.x + r * a.ld_bytes, a.v);
     const Kept k = load_kept(a, r, column_of(a, r), row);
+    const float c = kLog2e / a.temperature;
     Part p = no_part();
-    if ((int)threadIdx.x < a.parts) {
-        const uint64_t w = a.words[r * a.parts + threadIdx.x];
-        p.m = word_a(w);
-        p.s = word_b(w);
+    for (int i = threadIdx.x; i < a.parts; i += 64) {
+        const uint64_t w = a.words[r * a.parts + i];
+        p = merge(p, Part{word_a(w), word_b(w), 0.0f}, c);
     }
     float none;
-    finish_row<T>(a, r, k, wave_merge(p, kLog2e / a.temperature), none);
+    finish_row<T>(a, r, k, wave_merge(p, c), none);
 }
 
 // A wave a row while the row fits its registers; 256 lanes and 8 vectors beyond, or fewer vectors

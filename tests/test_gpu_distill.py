@@ -204,3 +204,24 @@ def test_calls_on_several_streams_at_once():
     for k, g in enumerate(got):
         for a, b in zip(g, want_h if k % 2 else want):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("tail,temperature", [("rest", 1.0), ("renorm", 1.0), ("renorm", 1.5)])
+@pytest.mark.parametrize("v,shift", [(524285, 0), (524286, 0), (524287, 0), (524288, 0), (524288, 1), (524286, 3), (524287, 2)])
+def test_the_longest_rows_to_their_end(v, shift, tail, temperature):
+    """Float32 rows of most columns, aligned or not: the student's mass lies in their last three columns, one of
+    which the teacher names."""
+    import ddm_amd
+    n, k = 3, 17
+    x, index, logprob = make(n, v, k, torch.float32, v + shift)
+    index[:] = torch.randint(0, v - 3, (n, k), generator=torch.Generator().manual_seed(v))
+    index[:, 3] = v - 1 - torch.arange(n)
+    x[:, -3:] = torch.tensor([12.0, 14.0, 13.0])
+    flat = torch.zeros(shift + n * v, device="cuda")
+    view = flat[shift:].view(n, v)
+    view.copy_(x)
+    args = (view, index.cuda(), logprob.cuda())
+    loss, _ = ddm_amd.topk_distill(*args, tail=tail, temperature=temperature)
+    both, grad = ddm_amd.topk_distill(*args, tail=tail, temperature=temperature, grad=True)
+    check(x, index, logprob, tail, temperature, None, loss, None)
+    check(x, index, logprob, tail, temperature, None, both, grad)
