@@ -126,7 +126,10 @@ __device__ __forceinline__ Gate gate_of(float l) {
     Gate g;
     g.a = __builtin_amdgcn_exp2f(l * 1.4426950408889634f);
     g.f = SCALE == DDM_GATED_NONE ? 1.0f : one_minus_exp(l, g.a);
-    if (SCALE == DDM_GATED_UNIT) g.f = __builtin_amdgcn_sqrtf(fmaxf(fmaf(g.f, g.a, g.f), 0.0f));    // (1 - a)(1 + a)
+    if (SCALE == DDM_GATED_UNIT) {
+        const float y = fmaf(g.f, g.a, g.f);                    // (1 - a)(1 + a)
+        g.f = __builtin_amdgcn_sqrtf(y < 0.0f ? 0.0f : y);      // a NaN gate's stays NaN (a maximum would drop it)
+    }
     return g;
 }
 // The factor's derivative by l.

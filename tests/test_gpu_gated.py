@@ -348,3 +348,52 @@ def test_beyond_four_gigabytes():
     assert (dx[first:].float() - fx.float()).abs().max() < 2.0 ** -4
     assert (dl[first:].float() - fl.float()).abs().max() / fl.float().abs().max() < 2.0 ** -7
 
+
+
+def nan_gates(x, lam, off, rows, channels):
+    """The inputs with NaN for the gates of `rows`, and what float64 makes of them."""
+    lam = lam.clone()
+    for r in rows:
+        lam[r, channels] = math.nan
+    return x, lam, off
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("d,g", [(64, 64), (5, 5), (96, 6)])
+@pytest.mark.parametrize("scale", ["none", "ewma", "unit"])
+@pytest.mark.parametrize("where", [1, 40, -1])
+def test_a_nan_gate_shows_wherever_it_counts(dtype, d, g, scale, where):
+    """One in a sequence's second row, further on, and in its last: in h from there on, in the state after, in the
+    gradients that it enters, and in nothing else."""
+    x, lam, off, state = make(900, d, g, dtype, dtype, 21, 4)
+    a, b = int(off[3]), int(off[4])
+    assert b - a > 45
+    x, lam, off = nan_gates(x, lam, off, [a + where if where > 0 else b - 1], slice(0, g, 2))
+    check(x, lam, off, state, scale, True)
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("scale", ["ewma", "unit"])
+def test_a_nan_gates_factor_without_a_state(dtype, scale):
+    """The first row has no state that a NaN gate could meet; the input's factor is NaN all the same."""
+    import ddm_amd
+    x, lam, off, _ = make(300, 32, 32, dtype, dtype, 22, 4, state=False)
+    lam[int(off[3]), ::3] = math.nan
+    gen = torch.Generator().manual_seed(0)
+    d_h, d_state = torch.randn(x.shape, generator=gen).to(dtype), torch.randn(4, 32, generator=gen)
+    xc, lc, oc = on(x, lam, off)
+    h, after = ddm_amd.gated_scan(xc, lc, offsets=oc, scale=scale)
+    got = ddm_amd.gated_scan_grad(xc, lc, h, d_h.cuda(), offsets=oc, d_state=d_state.cuda(), scale=scale)
+    ref = gated64(x, lam, off, None, scale, h.cpu(), d_h, d_state)
+    close(h, *ref["h"], dtype)
+    close(after, *ref["state"])
+    close(got[0], *ref["d_x"], dtype)
+    close(got[2], *ref["d_state"])
+    # At a log gate of -50, a^2 = e^-100 lies under float32's normal numbers: rounding it is off by 2^-150 and not by a
+    # share of it, so is rounding its product with x, and both are multiplied by the gradient (f = 1 there: d_x).
+    want, tol = ref["d_log_a"]
+    close(got[1], want, tol + 2.0 ** -150 * (x.double().abs() + 1) * ref["d_x"][0].abs(), dtype)
+    h, after = ddm_amd.gated_step(*on(x, lam), scale=scale)
+    ref = gated64(x, lam, torch.arange(301), None, scale)
+    close(h, *ref["h"], dtype)
+    close(after, *ref["state"])
