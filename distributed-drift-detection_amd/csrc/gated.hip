@@ -89,9 +89,9 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
             const bool in = active && inside >> r & 1, first = begins >> r & 1;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                if (in && first && a.state_in) {
+                if (in && first) {                   // without a state as well: a NaN gate's 0 is NaN
                     const int64_t s = a.off ? m.begins[tg * R + r] : 0;
-                    b[r][v] = fmaf(g[r][v % G], a.state_in[s * a.d + c + v], b[r][v]);
+                    b[r][v] = fmaf(g[r][v % G], a.state_in ? a.state_in[s * a.d + c + v] : 0.0f, b[r][v]);
                 }
                 if (!in) b[r][v] = 0.0f;
             }

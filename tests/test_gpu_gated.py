@@ -397,3 +397,18 @@ def test_a_nan_gates_factor_without_a_state(dtype, scale):
     ref = gated64(x, lam, torch.arange(301), None, scale)
     close(h, *ref["h"], dtype)
     close(after, *ref["state"])
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("seqs", [None, 4])
+def test_a_nan_gate_in_a_first_row_without_a_state(dtype, seqs):
+    """NaN times a state of 0 is NaN, in the scan as in the step, though nothing but the gate says so."""
+    import ddm_amd
+    x, lam, off, _ = make(300, 40, 20, dtype, dtype, 23, seqs, state=False)
+    first = 0 if off is None else int(off[3])
+    lam[first, 1::4] = math.nan
+    check(x, lam, off, None, "none", True)
+    h, after = ddm_amd.gated_step(*on(x, lam))
+    assert torch.equal(h[first].isnan().cpu(), lam[first].isnan().repeat_interleave(2))
+    one, state = ddm_amd.gated_scan(*on(x[first:first + 1], lam[first:first + 1]))
+    assert torch.equal(one[0].isnan(), h[first].isnan()) and torch.equal(state[0].isnan(), after[first].isnan())
