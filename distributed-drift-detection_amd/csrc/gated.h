@@ -132,6 +132,19 @@ __device__ __forceinline__ Gate gate_of(float l) {
     }
     return g;
 }
+// Gates are at most 1: products of theirs, which tiles and groups compose before they know the state, then
+// cannot overflow where the recurrence itself would not.  One over 1 counts as NaN, so that what it reaches
+// shows it.  (The scan asks first whether a wave has any: a select an entry took float32 scans
+// from three workgroups a CU to two, and others spilled.)
+template <int SCALE>
+__device__ __forceinline__ Gate bounded_gate_of(float l) {
+    Gate g = gate_of<SCALE>(l);
+    if (g.a > 1.0f) {
+        g.a = __builtin_nanf("");
+        if (SCALE != DDM_GATED_NONE) g.f = g.a;
+    }
+    return g;
+}
 // The factor's derivative by l.
 template <int SCALE>
 __device__ __forceinline__ float slope_of(const Gate& g) {

@@ -56,13 +56,12 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     }
     begins &= inside;
     ends &= inside;
-    const bool plain = !__any(active && (begins || ends || inside != (1u << R) - 1u));
-
     constexpr int G = OWN ? VEC : 1;                 // gates a lane; a cut is one of all its channels
     float g[R][G], b[R][VEC];
     Step own[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
+    uint64_t over = 0;                               // lanes with a gate over 1
     with_scale(a.scale, [&](auto scale) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -71,6 +70,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
             for (int k = 0; k < G; ++k) {
                 const Gate q = gate_of<scale()>(l[r][k]);
                 g[r][k] = q.a;
+                over |= __ballot(q.a > 1.0f);
                 in[k] = q.f;
             }
 #pragma unroll
@@ -81,12 +81,16 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
             }
         }
     });
+    const bool plain = !__any(active && (begins || ends || inside != (1u << R) - 1u)) && !(over & __ballot(active));
     if (!plain) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) own[v] = Step{1.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool in = active && inside >> r & 1, first = begins >> r & 1;
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+                if (g[r][k] > 1.0f) g[r][k] = __builtin_nanf("");
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 if (in && first) {                   // without a state as well: a NaN gate's 0 is NaN
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(256) void k_gated_step(Args a) {
     with_scale(a.scale, [&](auto scale) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const Gate q = gate_of<scale()>(l[v]);
+            const Gate q = bounded_gate_of<scale()>(l[v]);
             h[v] = fmaf(q.a, h[v], q.f * x[v]);
         }
     });

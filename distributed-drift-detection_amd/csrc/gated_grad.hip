@@ -69,7 +69,7 @@ __global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
     for (int r = R - 1; r >= 0; --r)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float g = gate_of<DDM_GATED_NONE>(l[r][v]).a, y = dh[r][v];
+            const float g = bounded_gate_of<DDM_GATED_NONE>(l[r][v]).a, y = dh[r][v];
             if (plain) {
                 own[v].a *= g;
                 own[v].b = g * (own[v].b + y);
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
                 float dx[VEC], dl[VEC];
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const Gate q = gate_of<scale()>(l[r][v]);
+                    const Gate q = bounded_gate_of<scale()>(l[r][v]);
                     const float grad = dh[r][v] + u[v];
                     dx[v] = grad * q.f;
                     dl[v] = grad * fmaf(slope_of<scale()>(q), x[r][v], q.a * hp[r][v]);
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
                     u[v] = 0.0f;
                     continue;
                 }
-                const Gate q = gate_of<scale()>(l[r][v]);
+                const Gate q = bounded_gate_of<scale()>(l[r][v]);
                 const float grad = dh[r][v] + (ends >> r & 1 ? given(r, v) : u[v]);
                 float before = hp[r][v];
                 u[v] = q.a * grad;

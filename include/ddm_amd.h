@@ -799,7 +799,8 @@ int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, int64_t v, in
  * to state_out[s][d], another buffer.  scale:
  *   DDM_GATED_NONE  b = x      DDM_GATED_EWMA  b = (1 - a) x      DDM_GATED_UNIT  b = sqrt(1 - a^2) x
  * log_a [rows][gates] (of x's type or float32; row stride 0: the same gates in every row), gates
- * dividing d: channel c has gate c / (d / gates).  out [rows][d] in x's type, the recurrence itself
+ * dividing d: channel c has gate c / (d / gates).  Log gates are at most 0; a gate over 1 counts as
+ * NaN, in the gradient and the step as well.  out [rows][d] in x's type, the recurrence itself
  * in float32.  Rows of no sequence are left alone, or zeroed (fill).  A sequence without rows
  * hands its state through.  Results do not depend on timing: the order of every composition is
  * fixed by the sizes.  scratch: ddm_gated_scan_scratch_bytes(...) bytes, 16-byte aligned, for one

@@ -412,3 +412,30 @@ def test_a_nan_gate_in_a_first_row_without_a_state(dtype, seqs):
     assert torch.equal(h[first].isnan().cpu(), lam[first].isnan().repeat_interleave(2))
     one, state = ddm_amd.gated_scan(*on(x[first:first + 1], lam[first:first + 1]))
     assert torch.equal(one[0].isnan(), h[first].isnan()) and torch.equal(state[0].isnan(), after[first].isnan())
+
+
+@pytest.mark.parametrize("dtype", [F, B, H])
+@pytest.mark.parametrize("scale", ["none", "ewma", "unit"])
+@pytest.mark.parametrize("value", [2.0 ** -22, 0.5, 60.0, math.inf])
+def test_a_gate_over_one_counts_as_nan(dtype, scale, value):
+    """Products of gates over 1 can overflow where the recurrence is finite (a state of 0), so there are none."""
+    import ddm_amd
+    x, lam, off, state = make(4000, 24, 12, dtype, dtype, 25, 5)
+    at = [0, int(off[3]), int(off[4]) + 70, int(off[4]) + 71, 3999]
+    x[int(off[4]):] = 0.0
+    above, nan = lam.clone(), lam.clone()
+    above[at, 1::3] = value
+    nan[at, 1::3] = math.nan
+    assert (above[at, 1::3] > 0).all()
+    d_h = torch.randn(4000, 24, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    xc, oc, sc = on(x, off, state)
+
+    def both(gates):
+        h, after = ddm_amd.gated_scan(xc, gates, offsets=oc, state=sc, scale=scale)
+        few = [0, int(off[3]), 3999]
+        step = ddm_amd.gated_step(xc[few], gates[few], scale=scale)
+        return (h, after) + ddm_amd.gated_scan_grad(xc, gates, h, d_h, offsets=oc, state=sc, scale=scale) + step
+    for a, b in zip(both(above.cuda()), both(nan.cuda())):
+        assert torch.equal(a.isnan(), b.isnan()) and a.isnan().any()
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    assert both(torch.zeros_like(lam).cuda())[0].isfinite().all()           # 0 itself is a gate of 1
