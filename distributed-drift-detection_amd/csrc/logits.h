@@ -215,7 +215,8 @@ __device__ __forceinline__ void add_vector(Lane& l, const float (&f)[N], float m
         if (most > l.limit) {
             to.m = fmaxf(l.m, most);
             to.scaled = fminf(fmaxf(to.m * c, -3e38f), 3e38f);
-            to.limit = fabsf(to.scaled) > kWide ? -INFINITY : to.m + 8.0f / c;
+            // finite, so that +inf exceeds it at any temperature and leaves its NaN
+            to.limit = fabsf(to.scaled) > kWide ? -INFINITY : fminf(to.m + 8.0f / c, FLT_MAX);
         }
         float d = l.scaled - to.scaled;
         if (__any(fabsf(l.scaled) > kWide || fabsf(to.scaled) > kWide))

@@ -225,3 +225,20 @@ def test_the_longest_rows_to_their_end(v, shift, tail, temperature):
     both, grad = ddm_amd.topk_distill(*args, tail=tail, temperature=temperature, grad=True)
     check(x, index, logprob, tail, temperature, None, loss, None)
     check(x, index, logprob, tail, temperature, None, both, grad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [2.0, 6e37, 3e38])
+@pytest.mark.parametrize("v", [2000, 4001, 40000])
+def test_students_with_infinity_at_huge_temperatures(dtype, temperature, v):
+    import ddm_amd
+    x, index, logprob = make(11, v, 9, dtype, 5)
+    x[0, v - 1] = x[2, v // 2] = math.inf
+    loss, grad = ddm_amd.topk_distill(x.cuda(), index.cuda(), logprob.cuda(), tail="renorm", temperature=temperature,
+                                      grad=True)
+    alone, _ = ddm_amd.topk_distill(x.cuda(), index.cuda(), logprob.cuda(), tail="renorm", temperature=temperature)
+    want = distill64(x, index, logprob, "renorm", temperature)
+    assert loss[[0, 2]].isnan().all() and alone[[0, 2]].isnan().all() and grad[[0, 2]].isnan().all()
+    sound = [r for r in range(11) if r not in (0, 2)]
+    close(loss[sound], want[0][sound], want[1][sound])
+    close(alone[sound], want[0][sound], want[1][sound])

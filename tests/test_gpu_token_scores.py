@@ -330,3 +330,17 @@ def test_the_longest_rows_to_their_end(v, shift, top):
     d = torch.randn(n, generator=g)
     want, tol = scores_grad64(x, t, ref, 1.0, d_logprob=d, d_entropy=d)
     close(ddm_amd.token_scores_grad(view, t.cuda(), r, d_logprob=d.cuda(), d_entropy=d.cuda()), want, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1.0, 3e37, 6e37, 3e38])
+@pytest.mark.parametrize("v", [2000, 4001, 40000])
+def test_rows_with_infinity_at_huge_temperatures(dtype, temperature, v):
+    """+inf behind finite entries of its lane, and before them: NaN, rank and indexes -1, error 1."""
+    import ddm_amd
+    x, t = make(12, v, dtype, 7, special=False)
+    x[1, v - 1] = x[3, 0] = x[5, v // 2] = math.inf
+    x[7, v - 1000] = math.nan
+    for n in (12, 8):
+        r = ddm_amd.token_scores(x[:n].cuda(), t[:n].cuda(), top=6, temperature=temperature)
+        check_scores(x[:n], t[:n], 6, temperature, r)
