@@ -192,7 +192,11 @@ __device__ __forceinline__ void gradient(float (&f)[N], float c, const Writer& w
 
 __device__ __forceinline__ uint64_t wait_for(const uint64_t* p) {
     uint64_t w = peek(p);
-    for (uint32_t spin = 0; w == kUnset && spin < kSpinLimit; ++spin) {
+    for (uint32_t looks = 0; w == kUnset; ++looks) {
+        if (looks == *(volatile uint32_t*)&guard.looks) {
+            tell_gave_up();
+            break;
+        }
         __builtin_amdgcn_s_sleep(1);
         w = peek(p);
     }
@@ -312,6 +316,8 @@ inline Shape distill_shape(int64_t n, int64_t nvec) {
 inline int64_t distill_scratch(const Shape& s, int64_t n) { return s.parts == 1 ? 0 : kTicketBytes + 8 * n * (s.parts + 2); }
 
 }  // namespace logits
+
+int use_guard_distill(const uint32_t* looks, bool* gave_up) { return use_guard(looks, gave_up); }
 }  // namespace ddm
 
 using namespace ddm;

@@ -258,21 +258,25 @@ struct ScanLds {
 // The first `count` (at most N) words of a column, all asked for at once; unset ones, if the guard
 // ever ran out, are NaN.
 template <int N>
-__device__ __forceinline__ void await(const uint64_t* p, int64_t stride, int count, uint64_t (&w)[N]) {
-    for (uint32_t spin = 0;; ++spin) {
+__device__ __forceinline__ void await(const uint64_t* p, int64_t stride, int count, uint64_t (&w)[N], bool& gave_up) {
+    for (uint32_t looks = 0;; ++looks) {
         bool set = true;
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = i < count ? peek(p + i * stride) : 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) set = set && w[i] != kUnset;
-        if (set || spin == kSpinLimit) return;
+        if (set) return;
+        if (looks == kLooks) {
+            gave_up = true;
+            return;
+        }
         __builtin_amdgcn_s_sleep(1);
     }
 }
 
-__device__ __forceinline__ uint64_t await_one(const uint64_t* p) {
+__device__ __forceinline__ uint64_t await_one(const uint64_t* p, bool& gave_up) {
     uint64_t w[1];
-    await<1>(p, 0, 1, w);
+    await<1>(p, 0, 1, w, gave_up);
     return w[0];
 }
 
@@ -280,40 +284,42 @@ __device__ __forceinline__ uint64_t await_one(const uint64_t* p) {
 // a group, whose last one publishes the group's step; as many groups form a row, and the state after
 // those is passed on one by one.  (Groups of 16 that pass the state on themselves: 1000003 x 32 bf16
 // 95 us, now 71; 200000 x 17 f32 with the gradient 101, now 80.  Rows of 16 groups of 16: 77 and 85.)
-__device__ __forceinline__ Step thread_steps(const uint64_t* p, int64_t stride, int count) {
+__device__ __forceinline__ Step thread_steps(const uint64_t* p, int64_t stride, int count, bool& gave_up) {
     Step s{1.0f, 0.0f};
     for (int j = 0; j < count; j += 4) {
         uint64_t w[4];
-        await<4>(p + j * stride, stride, count - j, w);
+        await<4>(p + j * stride, stride, count - j, w, gave_up);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (j + i < count) s = after(s, Step{word_a(w[i]), word_b(w[i])});
     }
     return s;
 }
-__device__ __forceinline__ float carry_of_thread(const Args& a, int64_t tile, int64_t c, const Step& all) {
+__device__ __forceinline__ float carry_of_thread(const Args& a, int64_t tile, int64_t c, const Step& all,
+                                                 bool& gave_up) {
     const int64_t g = tile / a.group, h = g / a.group;
     const int in_group = (int)(tile % a.group), in_groups = (int)(g % a.group);
     const bool last = in_group == a.group - 1, more = tile + 1 < a.ntiles;
     if (!last && more) publish(a.agg + tile * a.dp + c, word(all.a, all.b));
-    const Step tiles = thread_steps(a.agg + g * a.group * a.dp + c, a.dp, in_group);
+    const Step tiles = thread_steps(a.agg + g * a.group * a.dp + c, a.dp, in_group, gave_up);
     if (last && more) {
         const Step group = after(tiles, all);
         publish(a.inc + g * a.dp + c, word(group.a, group.b));
     }
-    const Step groups = thread_steps(a.inc + h * a.group * a.dp + c, a.dp, in_groups);
-    const float carry = apply(tiles, apply(groups, h > 0 ? word_a(await_one(a.far + (h - 1) * a.dp + c)) : 0.0f));
+    const Step groups = thread_steps(a.inc + h * a.group * a.dp + c, a.dp, in_groups, gave_up);
+    const float row = h > 0 ? word_a(await_one(a.far + (h - 1) * a.dp + c, gave_up)) : 0.0f;
+    const float carry = apply(tiles, apply(groups, row));
     if (last && in_groups == a.group - 1 && more) publish(a.far + h * a.dp + c, word(apply(all, carry), 0.0f));
     return carry;
 }
 
 // The same for one channel a wave, where there are few: a lane for each tile before in the group, then
 // a lane for each group before; groups and rows are of 64.
-__device__ __forceinline__ Step wave_steps(const uint64_t* p, int64_t stride, int count) {
+__device__ __forceinline__ Step wave_steps(const uint64_t* p, int64_t stride, int count, bool& gave_up) {
     const int lane = threadIdx.x & 63;
     Step s{1.0f, 0.0f};
     if (lane < count) {
-        const uint64_t w = await_one(p + lane * stride);
+        const uint64_t w = await_one(p + lane * stride, gave_up);
         s = Step{word_a(w), word_b(w)};
     }
 #pragma unroll
@@ -323,16 +329,18 @@ __device__ __forceinline__ Step wave_steps(const uint64_t* p, int64_t stride, in
     }
     return Step{__shfl(s.a, 0), __shfl(s.b, 0)};
 }
-__device__ __forceinline__ float carry_of_wave(const Args& a, int64_t tile, int64_t c, const Step& all) {
+__device__ __forceinline__ float carry_of_wave(const Args& a, int64_t tile, int64_t c, const Step& all,
+                                               bool& gave_up) {
     const int64_t g = tile / 64, h = g / 64;
     const int in_group = (int)(tile % 64), in_groups = (int)(g % 64);
     const bool first = (threadIdx.x & 63) == 0, last = in_group == 63, more = tile + 1 < a.ntiles;
     if (first && !last && more) publish(a.agg + tile * a.dp + c, word(all.a, all.b));
-    const Step tiles = wave_steps(a.agg + g * 64 * a.dp + c, a.dp, in_group);
+    const Step tiles = wave_steps(a.agg + g * 64 * a.dp + c, a.dp, in_group, gave_up);
     const Step group = after(tiles, all);
     if (first && last && more) publish(a.inc + g * a.dp + c, word(group.a, group.b));
-    const Step groups = wave_steps(a.inc + h * 64 * a.dp + c, a.dp, in_groups);
-    const float carry = apply(tiles, apply(groups, h > 0 ? word_a(await_one(a.far + (h - 1) * a.dp + c)) : 0.0f));
+    const Step groups = wave_steps(a.inc + h * 64 * a.dp + c, a.dp, in_groups, gave_up);
+    const float row = h > 0 ? word_a(await_one(a.far + (h - 1) * a.dp + c, gave_up)) : 0.0f;
+    const float carry = apply(tiles, apply(groups, row));
     if (first && last && in_groups == 63 && more) publish(a.far + h * a.dp + c, word(apply(all, carry), 0.0f));
     return carry;
 }
@@ -342,6 +350,7 @@ __device__ __forceinline__ float carry_of_wave(const Args& a, int64_t tile, int6
 template <int VEC>
 __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step (&own)[VEC], ScanLds<VEC>& l,
                                       float (&h)[VEC]) {
+    bool gave_up = false;
     const int cl = 1 << a.cl_bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int cols = cl * VEC, mine = (lane & (cl - 1)) * VEC;
     Step s[VEC];
@@ -378,7 +387,7 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
         float carry = 0.0f;
         if (a.tickets) {
             const int64_t c = (int64_t)at.block * cols + col;
-            carry = waves ? carry_of_wave(a, at.tile, c, all) : carry_of_thread(a, at.tile, c, all);
+            carry = waves ? carry_of_wave(a, at.tile, c, all, gave_up) : carry_of_thread(a, at.tile, c, all, gave_up);
         }
 #pragma unroll 2
         for (int w = 0; w < W; ++w) {
@@ -393,6 +402,7 @@ __device__ __forceinline__ void chain(const Args& a, const Place& at, const Step
         h[v] = l.b[wave][mine + v];
         if (cl < 64) h[v] = apply(s[v], h[v]);
     }
+    if (gave_up) tell_gave_up();             // here, where registers are free
 }
 
 // A lane's entries of a row: the row's address is the same in all lanes, and each lane's offset from

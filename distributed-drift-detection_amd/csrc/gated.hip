@@ -181,6 +181,8 @@ int begin(Args& a, const Shape& s, void* scratch, const float* from, float* to, 
 }
 
 }  // namespace gated
+
+int use_guard_gated(bool* gave_up) { return use_guard(nullptr, gave_up); }
 }  // namespace ddm
 
 using namespace ddm;

@@ -167,6 +167,8 @@ __global__ __launch_bounds__(256) void k_gated_sum(Args a, int64_t gates, int pe
 }
 
 }  // namespace gated
+
+int use_guard_gated_grad(bool* gave_up) { return use_guard(nullptr, gave_up); }
 }  // namespace ddm
 
 using namespace ddm;

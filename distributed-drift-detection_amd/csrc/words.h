@@ -7,7 +7,6 @@
 namespace ddm {
 
 constexpr uint64_t kUnset = ~0ull;
-constexpr uint32_t kSpinLimit = 1u << 22;      // some seconds: a guard, not a wait
 
 __device__ __forceinline__ uint64_t word(float a, float b) {
     const uint64_t w = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
@@ -21,6 +20,33 @@ __device__ __forceinline__ void publish(uint64_t* p, uint64_t w) {
 __device__ __forceinline__ uint64_t peek(const uint64_t* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+
+// A wait gives up after some seconds: a guard against a hang, not a wait.  What was waited for is NaN then, and so
+// is what follows from it, and the guard says that it was not the inputs'.  Every source that waits has one.
+// The recurrence's waits take the limit as a constant and tell the guard only after the last of them: in the
+// wait, either spilled registers (65536 x 2048 bf16 with float32 gates, gradient 570 us instead of 529).
+// The distillation's read it, so that a test can set it.
+constexpr uint32_t kLooks = 1u << 22;
+struct Guard {
+    uint32_t looks, gave_up;                   // at most; 1 once a wait took them all
+};
+[[maybe_unused]] static __device__ Guard guard = {kLooks, 0u};
+__device__ __forceinline__ void tell_gave_up() { *(volatile uint32_t*)&guard.gave_up = 1u; }
+// The current device's: a new limit (NULL: as it is), and whether a wait gave up since this was last asked (NULL: not
+// asked).  After hipDeviceSynchronize.
+[[maybe_unused]] static int use_guard(const uint32_t* looks, bool* gave_up) {
+    Guard g{};
+    if (int rc = hip_status(hipMemcpyFromSymbol(&g, HIP_SYMBOL(guard), sizeof g), "wait guard")) return rc;
+    if (gave_up) {
+        *gave_up = *gave_up || g.gave_up;
+        g.gave_up = 0;
+    }
+    if (looks) g.looks = *looks;
+    return hip_status(hipMemcpyToSymbol(HIP_SYMBOL(guard), &g, sizeof g), "wait guard");
+}
+int use_guard_distill(const uint32_t* looks, bool* gave_up);
+int use_guard_gated(bool* gave_up);
+int use_guard_gated_grad(bool* gave_up);
 // Queues of tickets: one counter gives out a ticket every 15 ns (measured: 32768 workgroups that took
 // one each ran no faster than that), so a launch has up to 8, 256 bytes apart, and a workgroup takes
 // from the queue that its index says.  What waits for each other is given out by one queue.

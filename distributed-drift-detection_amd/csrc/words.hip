@@ -22,3 +22,22 @@ int reset_words(uint32_t* tickets, uint64_t* words, int64_t nwords, const float*
 }
 
 }  // namespace ddm
+
+extern "C" int ddm_wait_gave_up(int32_t* gave_up) {
+    if (!gave_up) {
+        ddm::set_error("ddm_wait_gave_up: invalid argument (null pointer)");
+        return DDM_E_ARG;
+    }
+    bool any = false;
+    if (int rc = ddm::hip_status(hipDeviceSynchronize(), "ddm_wait_gave_up")) return rc;
+    if (int rc = ddm::use_guard_distill(nullptr, &any)) return rc;
+    if (int rc = ddm::use_guard_gated(&any)) return rc;
+    if (int rc = ddm::use_guard_gated_grad(&any)) return rc;
+    *gave_up = any;
+    return 0;
+}
+
+extern "C" int ddm_wait_limit(uint32_t looks) {
+    if (int rc = ddm::hip_status(hipDeviceSynchronize(), "ddm_wait_limit")) return rc;
+    return ddm::use_guard_distill(&looks, nullptr);
+}

@@ -16,7 +16,7 @@ _EXPORTS = {
     "run_DDM_loop": "controller", "run_partition_frame": "controller", "DevicePartition": "controller",
     "PartitionRunner": "controller", "DDMSettings": "params", "OUTPUT_COLUMNS": "params", "SCHEMA": "params",
     "token_scores": "tokens", "token_scores_grad": "tokens", "TokenScores": "tokens",
-    "topk_distill": "tokens", "gated_scan": "gated", "gated_scan_grad": "gated", "gated_step": "gated",
+    "topk_distill": "tokens", "gated_scan": "gated", "gated_scan_grad": "gated", "gated_step": "gated", "wait_gave_up": "_launch",
     "MTStream": "rng", "DdmError": "_capi", "lib": "_capi",
 }
 

@@ -12,7 +12,7 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 
 # DDM_AMD_LIB: an alternative build of the same library (e.g. an instrumented one)
 LIB_PATH = os.environ.get("DDM_AMD_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libddm_amd.so")
-ABI_VERSION = 25
+ABI_VERSION = 26
 
 DDM_E_ARG = 1001
 DDM_E_FOREST = 1002
@@ -167,6 +167,8 @@ SIGNATURES = {
                                            _vp]),
     "ddm_gated_step": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64,
                                       _vp, _vp, _vp]),
+    "ddm_wait_gave_up": (ctypes.c_int, [_vp]),
+    "ddm_wait_limit": (ctypes.c_int, [ctypes.c_uint32]),
     "ddm_synth_block_labels": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i32, _vp]),
     "ddm_synth_jitter_labels": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i32, ctypes.c_double, _u64,
                                                _vp]),

@@ -3,11 +3,12 @@
 A call on small operands costs the host more than the GPU, so the common case (the current
 stream of the current device) takes no context manager and makes no Stream object.
 """
+import ctypes
 import functools
 
 import torch
 
-from ._capi import lib
+from ._capi import check, lib
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -107,3 +108,14 @@ def overlap(a, b):
             apart, wide_a, wide_b = (b0 - a0) % row, a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
             return apart < wide_a or apart + wide_b > row
     return True
+
+
+def wait_gave_up(device=None):
+    """Whether a wait of one workgroup for another has given up on the device (None: the current one) since this was last
+    asked: no, unless something kept part of a launch from running for seconds.  Such a wait leaves NaN in the results of
+    `topk_distill` (with a gradient), `gated_scan` or `gated_scan_grad`; this tells it from a NaN of the inputs'.
+    Waits for the device's work so far."""
+    gave_up = ctypes.c_int32()
+    with torch.cuda.device(device):
+        check(lib.ddm_wait_gave_up(ctypes.byref(gave_up)), "ddm_wait_gave_up")
+    return bool(gave_up.value)

@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define DDM_AMD_ABI_VERSION 25
+#define DDM_AMD_ABI_VERSION 26
 
 #define DDM_E_ARG        1001   /* invalid argument (null pointer, bad size) */
 #define DDM_E_FOREST     1002   /* forest shape not supported (classes > 256) */
@@ -827,6 +827,14 @@ int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, const void* 
 int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const void* log_a, int32_t gate_dtype, int64_t ld_a,
                    int64_t rows, int64_t d, int64_t gates, int32_t scale, const float* state_in, float* state_out,
                    void* out, int64_t ld_out, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
+
+/* Workgroups of ddm_topk_distill (with a gradient) and of the gated scans wait for each other, for some
+ * seconds at most.  A wait that gives up leaves NaN; whether one did on the current device since this
+ * was last asked (the call waits for the device's work; not while a stream is captured). */
+int ddm_wait_gave_up(int32_t* gave_up);
+/* After how many looks a wait of ddm_topk_distill on the current device gives up, for tests of that path
+ * (2^22 when the library is loaded).  Waits for the device's work. */
+int ddm_wait_limit(uint32_t looks);
 
 /* ---- synthetic inputs (benchmark configs) ------------------------- */
 

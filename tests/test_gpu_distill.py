@@ -242,3 +242,20 @@ def test_students_with_infinity_at_huge_temperatures(dtype, temperature, v):
     sound = [r for r in range(11) if r not in (0, 2)]
     close(loss[sound], want[0][sound], want[1][sound])
     close(alone[sound], want[0][sound], want[1][sound])
+
+
+def test_a_wait_that_gives_up_says_so():
+    import ddm_amd
+    from ddm_amd import _capi
+    args = [t.cuda() for t in make(64, 60000, 16, torch.float32, 3)]
+    want = ddm_amd.topk_distill(*args, grad=True)
+    assert not ddm_amd.wait_gave_up()
+    _capi.check(_capi.lib.ddm_wait_limit(0), "limit")
+    try:
+        _, grad = ddm_amd.topk_distill(*args, grad=True)
+        assert ddm_amd.wait_gave_up() and (grad.isnan() & ~want[1].isnan()).any()
+    finally:
+        _capi.check(_capi.lib.ddm_wait_limit(1 << 22), "limit")
+    again = ddm_amd.topk_distill(*args, grad=True)
+    assert all(torch.equal(a.view(torch.int32), b.view(torch.int32)) for a, b in zip(again, want))
+    assert not ddm_amd.wait_gave_up()

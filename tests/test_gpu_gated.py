@@ -439,3 +439,16 @@ def test_a_gate_over_one_counts_as_nan(dtype, scale, value):
         assert torch.equal(a.isnan(), b.isnan()) and a.isnan().any()
         assert torch.equal(a.nan_to_num(), b.nan_to_num())
     assert both(torch.zeros_like(lam).cuda())[0].isfinite().all()           # 0 itself is a gate of 1
+
+
+def test_no_wait_gives_up():
+    """Hundreds of tiles that wait for each other, forwards and backwards, on two streams."""
+    import ddm_amd
+    x, lam, _, state = make(40000, 128, 128, B, B, 30)
+    args = on(x, lam, None, state)
+    h, _ = ddm_amd.gated_scan(*args)
+    torch.cuda.synchronize()
+    for stream in (None, torch.cuda.Stream()):
+        ddm_amd.gated_scan(*args, stream=stream)
+        ddm_amd.gated_scan_grad(args[0], args[1], h, h, state=args[3], stream=stream)
+    assert ddm_amd.wait_gave_up() is False and ddm_amd.wait_gave_up(0) is False

@@ -259,3 +259,7 @@ def test_columns_of_one_buffer_lie_apart():
         gated.gated_scan(cut(0, 20), cut(20, 30), out=cut(0, 20))
     with pytest.raises(ValueError, match="on the GPU"):
         tokens.token_scores_grad(cut(0, 10, slice(0, 4)), T, scores(), out=cut(10, 20, slice(0, 4)))
+
+
+def test_the_guards_state_needs_a_place():
+    assert _capi.lib.ddm_wait_gave_up(None) == _capi.DDM_E_ARG and "null" in last_error()
