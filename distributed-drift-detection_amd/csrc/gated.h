@@ -474,39 +474,46 @@ inline int wide_vec(int32_t dtype) { return 4 / elem_size(dtype); }
 // 4 bytes of x a lane (and a row) where every operand's rows are aligned for it and no such piece
 // has two gates; else an entry a lane.  Wider pieces would leave fewer rows to a lane's registers,
 // and so make more tiles of the same rows.
-inline int vec_of(int32_t dtype, int32_t gate_dtype, int d, int share, std::initializer_list<const void*> x,
-                  std::initializer_list<int64_t> ld, const void* l, int64_t ld_l, const void* dl, int64_t ld_dl) {
-    const int v = wide_vec(dtype), es = elem_size(dtype), gs = elem_size(gate_dtype);
+inline int vec_of(int32_t dtype, int32_t gate_dtype, int32_t h_dtype, int d, int share,
+                  std::initializer_list<const void*> x, std::initializer_list<int64_t> ld, const void* h, int64_t ld_h,
+                  const void* l, int64_t ld_l, const void* dl, int64_t ld_dl) {
+    const int v = wide_vec(dtype), es = elem_size(dtype), gs = elem_size(gate_dtype), hs = elem_size(h_dtype);
     if (v == 1 || d % v || (share > 1 && share % v)) return 1;
     for (const void* p : x)
         if ((uintptr_t)p % 4) return 1;
     for (int64_t s : ld)
         if (s * es % 4) return 1;
+    if ((uintptr_t)h % (v * hs) || ld_h * hs % (v * hs)) return 1;
     if (share == 1 && ((uintptr_t)l % (v * gs) || ld_l * gs % (v * gs) || (uintptr_t)dl % (v * gs) || ld_dl * gs % (v * gs)))
         return 1;
     return v;
 }
 
-// f(type of x, type of the gates, channels a lane, whether each has a gate of its own)
-template <typename X, typename L, typename F>
+// f(type of x, type of h, type of the gates, channels a lane, whether each has a gate of its own)
+template <typename X, typename H, typename L, typename F>
 void with_vec(int vec, bool own, F f) {
     if constexpr (sizeof(typename X::E) == 2) {
         using two = std::integral_constant<int, 2>;
-        if (vec == 2 && own) return f(X(), L(), two(), std::true_type());
-        if (vec == 2) return f(X(), L(), two(), std::false_type());
+        if (vec == 2 && own) return f(X(), H(), L(), two(), std::true_type());
+        if (vec == 2) return f(X(), H(), L(), two(), std::false_type());
     }
-    f(X(), L(), std::integral_constant<int, 1>(), std::false_type());      // its gate by its index
+    f(X(), H(), L(), std::integral_constant<int, 1>(), std::false_type());      // its gate by its index
+}
+template <typename X, typename F>
+void with_h(int32_t h_dtype, int32_t gate_dtype, int vec, bool own, F f) {
+    if (h_dtype == DDM_F32)
+        return gate_dtype == DDM_F32 ? with_vec<X, f32_t, f32_t>(vec, own, f) : with_vec<X, f32_t, X>(vec, own, f);
+    return gate_dtype == DDM_F32 ? with_vec<X, X, f32_t>(vec, own, f) : with_vec<X, X, X>(vec, own, f);
 }
 template <typename F>
-void with_types(int32_t dtype, int32_t gate_dtype, int vec, bool own, F f) {
-    if (dtype == DDM_F32) return with_vec<f32_t, f32_t>(vec, own, f);
-    if (dtype == DDM_BF16)
-        return gate_dtype == DDM_F32 ? with_vec<bf16_t, f32_t>(vec, own, f) : with_vec<bf16_t, bf16_t>(vec, own, f);
-    return gate_dtype == DDM_F32 ? with_vec<f16_t, f32_t>(vec, own, f) : with_vec<f16_t, f16_t>(vec, own, f);
+void with_types(int32_t dtype, int32_t h_dtype, int32_t gate_dtype, int vec, bool own, F f) {
+    if (dtype == DDM_F32) return with_vec<f32_t, f32_t, f32_t>(vec, own, f);
+    if (dtype == DDM_BF16) return with_h<bf16_t>(h_dtype, gate_dtype, vec, own, f);
+    return with_h<f16_t>(h_dtype, gate_dtype, vec, own, f);
 }
 
 inline int check(const char* who, int32_t dtype, int32_t gate_dtype, int64_t rows, int64_t d, int64_t gates,
-                 int64_t ld_x, int64_t ld_l, int64_t n, int32_t scale) {
+                 int64_t ld_x, int64_t ld_l, int64_t n, int32_t scale, int32_t flags) {
     if ((dtype != DDM_F32 && dtype != DDM_BF16 && dtype != DDM_F16) || (gate_dtype != dtype && gate_dtype != DDM_F32)) {
         set_error("%s: types %d and %d (gates of the inputs' type, or float32)", who, (int)dtype, (int)gate_dtype);
     } else if (rows < 0 || d < 1 || d > 1 << 20 || gates < 1 || d % gates || ld_x < d || (ld_l < gates && ld_l != 0) ||
@@ -515,6 +522,8 @@ inline int check(const char* who, int32_t dtype, int32_t gate_dtype, int64_t row
                   who, (long long)rows, (long long)d, (long long)gates, (long long)ld_x, (long long)ld_l);
     } else if (scale != DDM_GATED_NONE && scale != DDM_GATED_EWMA && scale != DDM_GATED_UNIT) {
         set_error("%s: unknown scale %d", who, (int)scale);
+    } else if (flags & ~(DDM_GATED_FILL | DDM_GATED_H_F32)) {
+        set_error("%s: unknown flags %d", who, (int)flags);
     } else {
         return 0;
     }

@@ -8,7 +8,7 @@ namespace gated {
 // 65536 x 2048 bf16, "unit", 37 sequences: 228 us, 3.5 TB/s; one sequence of them 207.  What is above
 // the 165 us of the same kernel without the chain is tiles waiting for tiles.  (With the steps computed
 // again after the wait, three workgroups fit a CU: "unit" 235 us, "none" no faster.)
-template <typename X, typename L, int VEC, bool OWN, int R>
+template <typename X, typename H, typename L, int VEC, bool OWN, int R>
 __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
@@ -23,7 +23,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     Raw<X, VEC> x[R];
     Gates<L, VEC, OWN> l[R];
     const uint32_t lane_x = tg * R * (uint32_t)a.ld_x + c * (uint32_t)sizeof(typename X::E);
-    const uint32_t lane_h = tg * R * (uint32_t)a.ld_h + c * (uint32_t)sizeof(typename X::E);
+    const uint32_t lane_h = tg * R * (uint32_t)a.ld_h + c * (uint32_t)sizeof(typename H::E);
     const uint32_t lane_l = tg * R * (uint32_t)a.ld_l + Gates<L, VEC, OWN>::column(a, c);
     const char *x0 = a.x + row0 * a.ld_x, *l0 = a.l + row0 * a.ld_l;
     char* h0 = a.out + row0 * a.ld_h;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
         for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) h[v] = fmaf(g[r][v % G], h[v], b[r][v]);
-            store<X, VEC>(h0 + r * a.ld_h, lane_h, h);
+            store<H, VEC>(h0 + r * a.ld_h, lane_h, h);
         }
         return;
     }
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {
     for (int r = 0; r < R; ++r) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) h[v] = apply(Step{g[r][v % G], b[r][v]}, h[v]);
-        if (active && (inside >> r & 1 || (a.fill && r0 + r < a.rows))) store<X, VEC>(h0 + r * a.ld_h, lane_h, h);
+        if (active && (inside >> r & 1 || (a.fill && r0 + r < a.rows))) store<H, VEC>(h0 + r * a.ld_h, lane_h, h);
         if (active && ends >> r & 1) {
             const int64_t s = a.off ? m.ends[tg * R + r] : 0;
 #pragma unroll
@@ -203,18 +203,19 @@ extern "C" int64_t ddm_gated_scan_scratch_bytes(int64_t rows, int64_t d, int64_t
 extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const void* log_a, int32_t gate_dtype,
                               int64_t ld_a, int64_t rows, int64_t d, int64_t gates, const int64_t* offsets, int64_t n,
                               int32_t scale, const float* state_in, float* state_out, void* out, int64_t ld_out,
-                              int32_t fill, void* scratch, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end) {
-    if (int rc = check("ddm_gated_scan", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, n, scale)) return rc;
+                              int32_t flags, void* scratch, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end) {
+    if (int rc = check("ddm_gated_scan", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, n, scale, flags)) return rc;
     if ((rows && (!x || !log_a || !out || ld_out < d)) || (n && !state_out) || (!offsets && n != 1) ||
         (state_in && state_in == state_out)) {
         set_error("ddm_gated_scan: invalid argument (null pointer, output stride, one sequence without offsets, or the "
                   "states in one buffer)");
         return DDM_E_ARG;
     }
-    const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype);
-    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
+    const int32_t h_dtype = flags & DDM_GATED_H_F32 ? DDM_F32 : dtype;
+    const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype), hs = elem_size(h_dtype);
+    const int vec = vec_of(dtype, gate_dtype, h_dtype, (int)d, share, {x}, {ld_x}, out, ld_out, log_a, ld_a, nullptr, 0);
     const Shape s = shape_of(rows, (int)d, share, vec, false);
-    if (int rc = check_tile("ddm_gated_scan", s, {ld_x * es, ld_a * gs, ld_out * es})) return rc;
+    if (int rc = check_tile("ddm_gated_scan", s, {ld_x * es, ld_a * gs, ld_out * hs})) return rc;
     if (scratch_bytes(s, rows, (int)d) && !scratch) {
         set_error("ddm_gated_scan: invalid argument (no scratch)");
         return DDM_E_ARG;
@@ -227,12 +228,12 @@ extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const 
         a.out = (char*)out;
         a.ld_x = ld_x * es;
         a.ld_l = ld_a * gs;
-        a.ld_h = ld_out * es;
+        a.ld_h = ld_out * hs;
         a.rows = rows;
         a.d = (int)d;
         a.share = share;
         a.scale = scale;
-        a.fill = fill;
+        a.fill = flags & DDM_GATED_FILL;
         a.off = offsets;
         a.n = n;
         a.state_in = state_in;
@@ -241,13 +242,14 @@ extern "C" int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const 
         if (rows == 0) return 0;
         const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
         const dim3 grid((unsigned)grid_of(a, s));
-        with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
+        with_types(dtype, h_dtype, gate_dtype, vec, share == 1, [&](auto xt, auto ht, auto lt, auto v, auto own) {
             using X = decltype(xt);
+            using H = decltype(ht);
             using L = decltype(lt);
             if (s.r == 16)
-                k_gated_scan<X, L, v(), own(), 16><<<grid, NT, lds, st>>>(a);
+                k_gated_scan<X, H, L, v(), own(), 16><<<grid, NT, lds, st>>>(a);
             else
-                k_gated_scan<X, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
+                k_gated_scan<X, H, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
         });
         return launch_status("ddm_gated_scan");
     });
@@ -257,7 +259,7 @@ extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const 
                               int64_t ld_a, int64_t rows, int64_t d, int64_t gates, int32_t scale, const float* state_in,
                               float* state_out, void* out, int64_t ld_out, ddm_stream_t stream, ddm_event_t ev_begin,
                               ddm_event_t ev_end) {
-    if (int rc = check("ddm_gated_step", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, rows, scale)) return rc;
+    if (int rc = check("ddm_gated_step", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, rows, scale, 0)) return rc;
     if (rows == 0) return 0;
     if (!x || !log_a || !state_out || !out || ld_out < d) {
         set_error("ddm_gated_step: invalid argument (null pointer or output stride)");
@@ -271,7 +273,7 @@ extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const 
         set_error("ddm_gated_step: the state after overlaps the inputs");
         return DDM_E_ARG;
     }
-    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, out}, {ld_x, ld_out}, log_a, ld_a, nullptr, 0);
+    const int vec = vec_of(dtype, gate_dtype, dtype, (int)d, share, {x}, {ld_x}, out, ld_out, log_a, ld_a, nullptr, 0);
     const int64_t blocks = ceil_div(rows * (d / vec), 256);
     if (int rc = check_grid("ddm_gated_step", blocks, 256)) return rc;
     const hipStream_t st = as_hip(stream);
@@ -289,7 +291,7 @@ extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const 
         a.scale = scale;
         a.state_in = state_in;
         a.state_out = state_out;
-        with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
+        with_types(dtype, dtype, gate_dtype, vec, share == 1, [&](auto xt, auto, auto lt, auto v, auto own) {
             k_gated_step<decltype(xt), decltype(lt), v(), own()><<<dim3((unsigned)blocks), 256, 0, st>>>(a);
         });
         return launch_status("ddm_gated_step");

@@ -8,8 +8,11 @@ namespace gated {
 // rows run from its last one back; bits of rows count from the first, as in the forward.  Four operands
 // a row leave room for 8 rows, and gates are computed again rather than kept, so three workgroups share
 // a CU.  65536 x 2048 bf16: 367 us, 4.4 TB/s; 16384 x 2048 bf16 with 128 gates: 94 us.
-template <typename X, typename L, int VEC, bool OWN, int R>
-__global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
+// h is of the inputs' type, half a step of which is then in the gates' gradients, or float32 (two workgroups
+// a CU, as many bytes again for a 16-bit h): the caller's choice.  16384 x 2048 bf16 with 128 gates, one
+// sequence: scan 49 -> 56 us, gradient 101 -> 123.
+template <typename X, typename H, typename L, int VEC, bool OWN, int R>
+__global__ __launch_bounds__(NT, (std::is_same<X, H>::value ? 6 : 4)) void k_gated_grad(Args a) {
     extern __shared__ int32_t marks[];
     __shared__ ScanLds<VEC> lds;
     const Place at = take(a);
@@ -21,17 +24,19 @@ __global__ __launch_bounds__(NT, 6) void k_gated_grad(Args a) {
     const bool active = c < a.d;
     Sequences seq{};
     if (a.off) seq = find_sequences(a, row0);
-    Raw<X, VEC> x[R], dh[R], hp[R];
+    Raw<X, VEC> x[R], dh[R];
+    Raw<H, VEC> hp[R];
     Gates<L, VEC, OWN> l[R];
     auto lane_of = [&](int64_t ld) { return tg * R * (uint32_t)ld + c * (uint32_t)sizeof(typename X::E); };
-    const uint32_t lane_x = lane_of(a.ld_x), lane_h = lane_of(a.ld_h), lane_dh = lane_of(a.ld_dh);
+    const uint32_t lane_x = lane_of(a.ld_x), lane_dh = lane_of(a.ld_dh);
+    const uint32_t lane_h = tg * R * (uint32_t)a.ld_h + c * (uint32_t)sizeof(typename H::E);
     const uint32_t column_l = Gates<L, VEC, OWN>::column(a, c), lane_l = tg * R * (uint32_t)a.ld_l + column_l;
     auto load_row = [&](int r) {
         const int64_t row = row0 + r;                 // of the first time group
         dh[r] = load<X, VEC>(a.dh + row * a.ld_dh, lane_dh);
         l[r].load_row(a.l + row * a.ld_l, lane_l);
         x[r] = load<X, VEC>(a.x + row * a.ld_x, lane_x);
-        if (r0 + r > 0) hp[r] = load<X, VEC>(a.h + (row - 1) * a.ld_h, lane_h);
+        if (r0 + r > 0) hp[r] = load<H, VEC>(a.h + (row - 1) * a.ld_h, lane_h);
     };
     if (row0 + tr <= a.rows) {
         if (active)
@@ -178,21 +183,22 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
                                    int64_t ld_a, const void* h, int64_t ld_h, const void* d_h, int64_t ld_dh,
                                    int64_t rows, int64_t d, int64_t gates, const int64_t* offsets, int64_t n,
                                    int32_t scale, const float* state_in, const float* d_state_out, float* d_state_in,
-                                   void* d_x, int64_t ld_dx, void* d_log_a, int64_t ld_da, int32_t fill, void* scratch,
+                                   void* d_x, int64_t ld_dx, void* d_log_a, int64_t ld_da, int32_t flags, void* scratch,
                                    ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end) {
-    if (int rc = check("ddm_gated_scan_grad", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, n, scale)) return rc;
+    if (int rc = check("ddm_gated_scan_grad", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, n, scale, flags)) return rc;
     if ((rows && (!x || !log_a || !h || !d_h || !d_x || !d_log_a || ld_h < d || ld_dh < d || ld_dx < d || ld_da < gates)) ||
         (n && !d_state_in) || (!offsets && n != 1) || (d_state_out && d_state_out == d_state_in)) {
         set_error("ddm_gated_scan_grad: invalid argument (null pointer, stride, one sequence without offsets, or the "
                   "states in one buffer)");
         return DDM_E_ARG;
     }
-    const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype);
-    const int vec = vec_of(dtype, gate_dtype, (int)d, share, {x, h, d_h, d_x}, {ld_x, ld_h, ld_dh, ld_dx}, log_a, ld_a,
-                           d_log_a, ld_da);
+    const int32_t h_dtype = flags & DDM_GATED_H_F32 ? DDM_F32 : dtype;
+    const int share = (int)(d / gates), es = elem_size(dtype), gs = elem_size(gate_dtype), hs = elem_size(h_dtype);
+    const int vec = vec_of(dtype, gate_dtype, h_dtype, (int)d, share, {x, d_h, d_x}, {ld_x, ld_dh, ld_dx}, h, ld_h, log_a,
+                           ld_a, d_log_a, ld_da);
     const Shape s = shape_of(rows, (int)d, share, vec, true);
     if (int rc = check_tile("ddm_gated_scan_grad", s,
-                            {ld_x * es, ld_a * gs, ld_h * es, ld_dh * es, ld_dx * es, ld_da * gs}))
+                            {ld_x * es, ld_a * gs, ld_h * hs, ld_dh * es, ld_dx * es, ld_da * gs}))
         return rc;
     const int64_t sums = s.dl_parts ? ceil_div(rows * gates, 256) : 0;
     if (int rc = check_grid("ddm_gated_scan_grad", sums, 256)) return rc;
@@ -211,7 +217,7 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
         a.dl = (char*)d_log_a;
         a.ld_x = ld_x * es;
         a.ld_l = ld_a * gs;
-        a.ld_h = ld_h * es;
+        a.ld_h = ld_h * hs;
         a.ld_dh = ld_dh * es;
         a.ld_dx = ld_dx * es;
         a.ld_dl = ld_da * gs;
@@ -219,7 +225,7 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
         a.d = (int)d;
         a.share = share;
         a.scale = scale;
-        a.fill = fill;
+        a.fill = flags & DDM_GATED_FILL;
         a.off = offsets;
         a.n = n;
         a.state_in = state_in;
@@ -230,13 +236,14 @@ extern "C" int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, c
         const size_t lds = offsets ? Marks::bytes((NT >> s.cl_bits) * s.r) : 0;
         const dim3 grid((unsigned)grid_of(a, s));
         int rc = 0;
-        with_types(dtype, gate_dtype, vec, share == 1, [&](auto xt, auto lt, auto v, auto own) {
+        with_types(dtype, h_dtype, gate_dtype, vec, share == 1, [&](auto xt, auto ht, auto lt, auto v, auto own) {
             using X = decltype(xt);
+            using H = decltype(ht);
             using L = decltype(lt);
             if (s.r == 8)
-                k_gated_grad<X, L, v(), own(), 8><<<grid, NT, lds, st>>>(a);
+                k_gated_grad<X, H, L, v(), own(), 8><<<grid, NT, lds, st>>>(a);
             else
-                k_gated_grad<X, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
+                k_gated_grad<X, H, L, v(), own(), 4><<<grid, NT, lds, st>>>(a);
             rc = launch_status("ddm_gated_scan_grad");
             if (!rc && sums) k_gated_sum<L><<<dim3((unsigned)sums), 256, 0, st>>>(a, gates, s.dl_parts);
         });

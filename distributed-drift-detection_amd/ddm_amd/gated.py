@@ -17,6 +17,14 @@ from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, sh
 from .kernels import _evs, _ptr
 
 SCALES = {"none": 0, "ewma": 1, "unit": 2}
+FILL, H_F32 = 1, 2
+
+
+def _h_type(name, t, x):
+    """Flag of an h of x's type or float32."""
+    if t not in (x.dtype, torch.float32):
+        raise TypeError(f"{name} has type {t}; supported: {x.dtype} (x's) or torch.float32")
+    return H_F32 if t == torch.float32 else 0
 
 
 def _scale(scale):
@@ -57,7 +65,7 @@ def _sequences(offsets, state, name, d):
     return n
 
 
-def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, stream=None, timer=None):
+def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, stream=None, timer=None, dtype=None):
     """h [rows, d] (x's type) and the state after every sequence [n, d] (float32) of
     h_t = exp(log_a_t) h_{t-1} + b_t, b = x ("none"), (1 - a) x ("ewma") or sqrt(1 - a^2) x ("unit").
 
@@ -66,15 +74,18 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
     offsets int64 [n + 1] on the device, not decreasing: sequence s is rows offsets[s] ..
     offsets[s+1] - 1 (None: one sequence of all rows).  state [n, d] float32: before the first rows
     (None: 0).  Rows of no sequence are zero in a new h and left alone in a given `out`, which
-    may be x itself.  NaN and infinities stay within their sequence and channel."""
+    may be x itself.  dtype (or out's): torch.float32 keeps h as it was computed, which gated_scan_grad makes the
+    gates' gradients of; None is x's type, and half the bytes of 16-bit inputs' h.  NaN and infinities stay within their sequence and channel."""
     rows, d, gates, ld_x, ld_a = _inputs(x, log_a)
     mode = _scale(scale)
     n = _sequences(offsets, state, "state", d)
+    dtype = dtype or (x.dtype if out is None else out.dtype)
+    flags = _h_type("h", dtype, x) | (FILL if out is None else 0)
     if out is not None:
         ld_out = rows_of("out", out)
-        if out.shape != x.shape or out.dtype != x.dtype:
-            raise ValueError(f"out must be {x.dtype} {list(x.shape)}, got {out.dtype} {list(out.shape)}")
-        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+        if out.shape != x.shape or out.dtype != dtype:
+            raise ValueError(f"out must be {dtype} {list(x.shape)}, got {out.dtype} {list(out.shape)}")
+        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and out.dtype == x.dtype
         for t in (x, log_a, offsets, state):
             if t is not None and overlap(out, t) and not (t is x and same):
                 raise ValueError("out overlaps an input without being x")
@@ -83,17 +94,17 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
     context, s = launch_on(x, stream, (x, log_a, offsets, state, out))
     with context:
         offsets, state = dense(offsets), dense(state)
-        h = torch.empty((rows, d), dtype=x.dtype, device=x.device) if out is None else out
+        h = torch.empty((rows, d), dtype=dtype, device=x.device) if out is None else out
         after = torch.empty((n, d), dtype=torch.float32, device=x.device)
         scratch = scratch_for(x.device, "ddm_gated_scan_scratch_bytes", rows, d, gates, DTYPES[x.dtype], 0)
         check(lib.ddm_gated_scan(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a, rows,
                                  d, gates, _ptr(offsets), n, mode, _ptr(state), after.data_ptr(), h.data_ptr(), ld_out,
-                                 out is None, _ptr(scratch), s, *_evs(timer)), "ddm_gated_scan")
+                                 flags, _ptr(scratch), s, *_evs(timer)), "ddm_gated_scan")
     return h, after
 
 
 def gated_scan_grad(x, log_a, h, d_h, offsets=None, state=None, d_state=None, scale="none", stream=None, timer=None):
-    """Gradients of a gated_scan that returned h: (d_x like x, d_log_a like log_a but dense, the
+    """Gradients of a gated_scan that returned h (x's type, or float32: see there): (d_x like x, d_log_a like log_a but dense, the
     gradient of `state` [n, d] float32) from d_h [rows, d] (x's type) and d_state [n, d] float32, the
     gradient of the state after (None: 0).  Rows of no sequence have gradient 0.  At a = 1 the
     "unit" factor's infinite slope counts as 0."""
@@ -103,8 +114,9 @@ def gated_scan_grad(x, log_a, h, d_h, offsets=None, state=None, d_state=None, sc
     strides = []
     for name, t in (("h", h), ("d_h", d_h)):
         strides.append(rows_of(name, t))
-        if t.shape != x.shape or t.dtype != x.dtype:
+        if t.shape != x.shape or t.dtype not in (x.dtype, torch.float32 if name == "h" else x.dtype):
             raise ValueError(f"{name} must be {x.dtype} {list(x.shape)}, got {t.dtype} {list(t.shape)}")
+    flags = _h_type("h", h.dtype, x) | FILL
     if d_state is not None:
         shaped("d_state", d_state, (n, d), torch.float32)
     context, s = launch_on(x, stream, (x, log_a, h, d_h, offsets, state, d_state))
@@ -117,7 +129,7 @@ def gated_scan_grad(x, log_a, h, d_h, offsets=None, state=None, d_state=None, sc
         check(lib.ddm_gated_scan_grad(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a,
                                       h.data_ptr(), strides[0], d_h.data_ptr(), strides[1], rows, d, gates,
                                       _ptr(offsets), n, mode, _ptr(state), _ptr(d_state), before.data_ptr(),
-                                      d_x.data_ptr(), d, d_a.data_ptr(), gates, 1, _ptr(scratch), s, *_evs(timer)),
+                                      d_x.data_ptr(), d, d_a.data_ptr(), gates, flags, _ptr(scratch), s, *_evs(timer)),
               "ddm_gated_scan_grad")
     return d_x, d_a, before
 

@@ -801,17 +801,20 @@ int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, int64_t v, in
  * log_a [rows][gates] (of x's type or float32; row stride 0: the same gates in every row), gates
  * dividing d: channel c has gate c / (d / gates).  Log gates are at most 0; a gate over 1 counts as
  * NaN, in the gradient and the step as well.  out [rows][d] in x's type, the recurrence itself
- * in float32.  Rows of no sequence are left alone, or zeroed (fill).  A sequence without rows
- * hands its state through.  Results do not depend on timing: the order of every composition is
+ * in float32.  flags: DDM_GATED_FILL zeroes rows of no sequence, which are left alone otherwise;
+ * DDM_GATED_H_F32: out (the gradient's h) is float32, so that no gate's gradient is made of a rounded
+ * state.  A sequence without rows hands its state through.  Results do not depend on timing: the order of every composition is
  * fixed by the sizes.  scratch: ddm_gated_scan_scratch_bytes(...) bytes, 16-byte aligned, for one
  * call at a time (NULL if 0). */
 #define DDM_GATED_NONE 0
 #define DDM_GATED_EWMA 1
 #define DDM_GATED_UNIT 2
+#define DDM_GATED_FILL  1
+#define DDM_GATED_H_F32 2
 int64_t ddm_gated_scan_scratch_bytes(int64_t rows, int64_t d, int64_t gates, int32_t dtype, int32_t grad);
 int ddm_gated_scan(const void* x, int32_t dtype, int64_t ld_x, const void* log_a, int32_t gate_dtype, int64_t ld_a,
                    int64_t rows, int64_t d, int64_t gates, const int64_t* offsets, int64_t n, int32_t scale,
-                   const float* state_in, float* state_out, void* out, int64_t ld_out, int32_t fill, void* scratch,
+                   const float* state_in, float* state_out, void* out, int64_t ld_out, int32_t flags, void* scratch,
                    ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end);
 /* Its gradient: d_h [rows][d] and d_state_out[n][d] (NULL: 0) in; d_x, d_log_a (in the types of x
  * and log_a) and d_state_in[n][d] out.  h is ddm_gated_scan's out; d_log_a sums over the channels
@@ -820,7 +823,7 @@ int ddm_gated_scan_grad(const void* x, int32_t dtype, int64_t ld_x, const void* 
                         const void* h, int64_t ld_h, const void* d_h, int64_t ld_dh, int64_t rows, int64_t d,
                         int64_t gates, const int64_t* offsets, int64_t n, int32_t scale, const float* state_in,
                         const float* d_state_out, float* d_state_in, void* d_x, int64_t ld_dx, void* d_log_a,
-                        int64_t ld_da, int32_t fill, void* scratch, ddm_stream_t stream, ddm_event_t ev_begin,
+                        int64_t ld_da, int32_t flags, void* scratch, ddm_stream_t stream, ddm_event_t ev_begin,
                         ddm_event_t ev_end);
 /* One row a sequence (row s continues state s); state_out may be state_in, and overlaps neither x
  * nor log_a. */

@@ -452,3 +452,70 @@ def test_no_wait_gives_up():
         ddm_amd.gated_scan(*args, stream=stream)
         ddm_amd.gated_scan_grad(args[0], args[1], h, h, state=args[3], stream=stream)
     assert ddm_amd.wait_gave_up() is False and ddm_amd.wait_gave_up(0) is False
+
+
+@pytest.mark.parametrize("dtype,gate_dtype", [(B, B), (B, F), (H, H), (H, F)])
+@pytest.mark.parametrize("rows,d,g,seqs", [(1, 3, 1, None), (500, 64, 64, 6), (900, 257, 257, 3), (1000, 260, 65, 4), (600, 768, 12, 5),
+                                           (9001, 2048, 32, 5), (70001, 256, 256, 3)])
+def test_float32_h(dtype, gate_dtype, rows, d, g, seqs):
+    """h as it was computed: no rounding of the state in it, nor in the gates' gradients."""
+    import ddm_amd
+    for k, scale in enumerate(("none", "ewma", "unit")):
+        x, lam, off, state = make(rows, d, g, dtype, gate_dtype, rows + d + 2 * k + 1, seqs)
+        xc, lc, oc, sc = on(x, lam, off, state)
+        h, after = ddm_amd.gated_scan(xc, lc, offsets=oc, state=sc, scale=scale, dtype=F)
+        assert h.dtype == F
+        d_h = torch.randn(x.shape, generator=torch.Generator().manual_seed(k)).to(dtype)
+        got = ddm_amd.gated_scan_grad(xc, lc, h, d_h.cuda(), offsets=oc, state=sc, scale=scale)
+        ref = gated64(x, lam, off, state, scale, h.cpu(), d_h)
+        close(h, *ref["h"])
+        close(after, *ref["state"])
+        close(got[0], *ref["d_x"], dtype)
+        close(got[1], *ref["d_log_a"], gate_dtype)
+        close(got[2], *ref["d_state"])
+        short, same = ddm_amd.gated_scan(xc, lc, offsets=oc, state=sc, scale=scale)
+        # not h.to(dtype) bit by bit: one instruction rounds a fused product to float16 at once, two round it twice;
+        # either is within the bound of h and half a step of the type
+        close(short, *ref["h"], dtype)
+        assert torch.equal(same, after)
+
+
+@pytest.mark.parametrize("dtype", [B, H])
+def test_a_gates_gradient_without_a_rounded_state(dtype):
+    """Float32 gates and h: d_log_a against the recurrence that is float64 throughout."""
+    import ddm_amd
+    x, lam, off, state = make(700, 96, 96, dtype, F, 41, 4)
+    d_h = torch.randn(x.shape, generator=torch.Generator().manual_seed(3)).to(dtype)
+    xc, lc, oc, sc = on(x, lam, off, state)
+    h, _ = ddm_amd.gated_scan(xc, lc, offsets=oc, state=sc, dtype=F)
+    _, d_a, _ = ddm_amd.gated_scan_grad(xc, lc, h, d_h.cuda(), offsets=oc, state=sc)
+    exact, bound = gated64(x, lam, off, state, "none")["h"]
+    ref = gated64(x, lam, off, state, "none", exact, d_h)
+    # d_log_a = grad a h_{t-1}, and grad is d_x here: h_{t-1} is off by its bound and half a step of float32
+    off_by = torch.zeros_like(bound)
+    off_by[1:] = (bound + 2.0 ** -24 * exact.abs())[:-1]
+    want, tol = ref["d_log_a"]
+    close(d_a, want, tol + ref["d_x"][0].abs() * lam.double().exp() * off_by)
+
+
+def test_float32_out_and_strides():
+    import ddm_amd
+    x, lam, off, state = make(600, 64, 64, B, B, 43, 5)
+    args = on(x, lam, off, state)
+    want, _ = ddm_amd.gated_scan(*args, scale="ewma", dtype=F)
+    a, b = int(off[0]), int(off[-1])
+    d_h = torch.randn(600, 64, device="cuda").to(B)
+    grads = ddm_amd.gated_scan_grad(args[0], args[1], want, d_h, offsets=args[2], state=args[3], scale="ewma")
+    for shift in (0, 1, 2):                              # a shift by one: no aligned pair of h
+        wide = torch.full((600, 70), 7.0, device="cuda")
+        out = wide[:, shift:shift + 64]
+        h, _ = ddm_amd.gated_scan(*args, scale="ewma", out=out)
+        assert h is out and (wide[:, :shift] == 7).all() and (wide[:, shift + 64:] == 7).all()
+        assert (h[:a] == 7).all() and (h[b:] == 7).all()
+        ref = gated64(x, lam, off, state, "ewma", h.cpu(), d_h.cpu())
+        close(h[a:b], *(t[a:b] for t in ref["h"]))
+        got = ddm_amd.gated_scan_grad(args[0], args[1], h, d_h, offsets=args[2], state=args[3], scale="ewma")
+        for t, name in zip(got, ("d_x", "d_log_a", "d_state")):
+            close(t, *ref[name], t.dtype)
+        if shift == 0:
+            assert all(torch.equal(t, u) for t, u in zip(got, grads))

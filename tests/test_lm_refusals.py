@@ -263,3 +263,26 @@ def test_columns_of_one_buffer_lie_apart():
 
 def test_the_guards_state_needs_a_place():
     assert _capi.lib.ddm_wait_gave_up(None) == _capi.DDM_E_ARG and "null" in last_error()
+
+
+def test_types_of_h():
+    x, g, f = X.to(torch.bfloat16), G.to(torch.bfloat16), torch.float32
+    for kw, error in (({"dtype": torch.float16}, "h has type"), ({"dtype": torch.float64}, "h has type"),
+                      ({"out": torch.zeros(4, 10, dtype=torch.float16)}, "h has type"),
+                      ({"out": X.clone(), "dtype": torch.bfloat16}, "out must be"), ({"out": X.clone()}, "on the GPU"),
+                      ({"dtype": f}, "on the GPU"), ({"dtype": f, "out": x}, "out must be")):
+        with pytest.raises((ValueError, TypeError), match=error):
+            gated.gated_scan(x, g, **kw)
+    base = torch.zeros(4, 20, dtype=torch.bfloat16)     # float32 results over the 16-bit inputs
+    with pytest.raises(ValueError, match="overlaps"):
+        gated.gated_scan(base[:, :10], g, out=base.view(f))
+    with pytest.raises(ValueError, match="on the GPU"):
+        gated.gated_scan_grad(x, g, X, x)
+    with pytest.raises(ValueError, match="h must"):
+        gated.gated_scan_grad(x, g, x.half(), x)
+    with pytest.raises(ValueError, match="d_h must"):
+        gated.gated_scan_grad(x, g, X, X)
+    one, two = ctypes.c_void_p(256), ctypes.c_void_p(512)
+    for flags in (4, -1):
+        assert _capi.lib.ddm_gated_scan(one, 1, 10, one, 1, 5, 4, 10, 5, one, 2, 0, None, two, one, 10, flags, None, None,
+                                        None, None) == _capi.DDM_E_ARG and "flags" in last_error()
