@@ -91,6 +91,12 @@ def dense(t):
     return None if t is None else t.contiguous()
 
 
+def written(t):
+    """The caller's `t` was overwritten: autograd refuses a backward pass that saved what it held."""
+    if t is not None and not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _span(t):
     if t.is_contiguous():
         return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()

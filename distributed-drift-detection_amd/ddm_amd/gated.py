@@ -8,12 +8,13 @@ entropies), with a gate a row, so that a row can also forget everything (log gat
 `gated_step` continues every sequence by one row.
 
 Calls are asynchronous on `stream` (default: the current stream of the inputs' device), read
-nothing back and can be captured; results do not change from run to run.
+nothing back and can be captured; results do not change from run to run.  They carry no autograd history,
+whether the inputs require a gradient or not.
 """
 import torch
 
 from ._capi import check, lib
-from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, shaped
+from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, shaped, written
 from .kernels import _evs, _ptr
 
 SCALES = {"none": 0, "ewma": 1, "unit": 2}
@@ -100,6 +101,7 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
         check(lib.ddm_gated_scan(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a, rows,
                                  d, gates, _ptr(offsets), n, mode, _ptr(state), after.data_ptr(), h.data_ptr(), ld_out,
                                  flags, _ptr(scratch), s, *_evs(timer)), "ddm_gated_scan")
+    written(out)
     return h, after
 
 
@@ -155,4 +157,5 @@ def gated_step(x, log_a, state=None, scale="none", out_state=None, stream=None, 
         check(lib.ddm_gated_step(x.data_ptr(), DTYPES[x.dtype], ld_x, log_a.data_ptr(), DTYPES[log_a.dtype], ld_a, rows,
                                  d, gates, mode, _ptr(state), after.data_ptr(), h.data_ptr(), d, s, *_evs(timer)),
               "ddm_gated_step")
+    written(out_state)
     return h, after

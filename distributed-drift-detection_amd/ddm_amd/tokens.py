@@ -7,14 +7,16 @@ pass.  `topk_distill` is the loss (and gradient) of train_rf's part (:98-105): a
 refitted on the alternatives another one gave.
 
 The calls are asynchronous on `stream` (default: the current stream of the logits' device),
-read nothing back and can be captured.  Results belong to that stream.
+read nothing back and can be captured.  Results belong to that stream.  They carry no autograd history, whether
+the logits require a gradient or not: the gradients are calls of their own (`logits.backward(gradient)`
+goes on from there).
 """
 import collections
 
 import torch
 
 from ._capi import check, lib
-from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, shaped
+from ._launch import DTYPES, dense, launch_on, overlap, rows_of, scratch_for, shaped, written
 from .kernels import _evs, _ptr
 
 MAX_COLUMNS = 1 << 19
@@ -112,6 +114,7 @@ def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d
         shaped("scores.top_index", index, (n, top), torch.int32)
         shaped("d_top", d_top, (n, top), torch.float32)
     _check_out(out, logits, targets, scores.stats, scores.entropy, index, d_logprob, d_entropy, d_top)
+    into = out
     given = (logits, targets, scores.stats, scores.entropy, index, d_logprob, d_entropy, d_top, out)
     context, s = launch_on(logits, stream, given)
     with context:
@@ -123,6 +126,7 @@ def token_scores_grad(logits, targets, scores, d_logprob=None, d_entropy=None, d
                                         entropy.data_ptr(), _ptr(index), _ptr(d_logprob), _ptr(d_entropy),
                                         _ptr(d_top), out.data_ptr(), out_ld, s, *_evs(timer)),
               "ddm_token_scores_grad")
+    written(into)
     return out
 
 
@@ -154,7 +158,7 @@ def topk_distill(logits, index, logprob, tail="rest", temperature=1.0, weight=No
     if weight is not None:
         shaped("weight", weight, (n,), torch.float32)
     _check_out(out, logits, index, logprob, weight)
-    code = DTYPES[logits.dtype]
+    into, code = out, DTYPES[logits.dtype]
     context, s = launch_on(logits, stream, (logits, index, logprob, weight, out))
     with context:
         index, logprob, weight = dense(index), dense(logprob), dense(weight)
@@ -165,4 +169,5 @@ def topk_distill(logits, index, logprob, tail="rest", temperature=1.0, weight=No
         check(lib.ddm_topk_distill(logits.data_ptr(), code, n, v, ld, index.data_ptr(), index.element_size(),
                                    logprob.data_ptr(), k, TAILS[tail], temperature, _ptr(weight), loss.data_ptr(),
                                    _ptr(out), out_ld, _ptr(scratch), s, *_evs(timer)), "ddm_topk_distill")
+    written(into)
     return loss, out

@@ -344,3 +344,35 @@ def test_rows_with_infinity_at_huge_temperatures(dtype, temperature, v):
     for n in (12, 8):
         r = ddm_amd.token_scores(x[:n].cuda(), t[:n].cuda(), top=6, temperature=temperature)
         check_scores(x[:n], t[:n], 6, temperature, r)
+
+
+def saved(make_buffer, write):
+    """Whether autograd refuses a backward pass whose saved tensor `write` has overwritten."""
+    leaf = make_buffer().requires_grad_()
+    buf = leaf * 1.0
+    total = buf.pow(2).sum()                            # keeps buf
+    write(buf.detach())
+    try:
+        total.backward()
+    except RuntimeError as e:
+        return "inplace" in str(e)
+    return False
+
+
+def test_results_over_saved_tensors():
+    import ddm_amd
+    n, v = 5, 300
+    t = torch.zeros(n, dtype=torch.int64, device="cuda")
+    x = torch.randn(n, v, device="cuda")
+    r = ddm_amd.token_scores(x, t, top=4)
+    d = torch.ones(n, device="cuda")
+    assert saved(x.clone, lambda b: ddm_amd.token_scores_grad(b, t, r, d_logprob=d, out=b))
+    assert saved(x.clone, lambda b: ddm_amd.token_scores_grad(x, t, r, d_logprob=d, out=b))
+    assert saved(x.clone, lambda b: ddm_amd.topk_distill(b, r.top_index, r.top_logprob, out=b))
+    assert saved(x.clone, lambda b: ddm_amd.gated_scan(b, -x.abs(), out=b))
+    assert saved(x.clone, lambda b: ddm_amd.gated_step(x, -x.abs(), b, out_state=b))
+    assert not saved(x.clone, lambda b: ddm_amd.token_scores_grad(b, t, r, d_logprob=d))
+    assert not saved(x.clone, lambda b: ddm_amd.gated_scan(b, -x.abs()))
+    with torch.inference_mode():
+        y = x.clone()
+        ddm_amd.token_scores_grad(y, t, r, d_logprob=d, out=y)

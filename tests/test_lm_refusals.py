@@ -286,3 +286,16 @@ def test_types_of_h():
     for flags in (4, -1):
         assert _capi.lib.ddm_gated_scan(one, 1, 10, one, 1, 5, 4, 10, 5, one, 2, 0, None, two, one, 10, flags, None, None,
                                         None, None) == _capi.DDM_E_ARG and "flags" in last_error()
+
+
+def test_what_was_written_counts_as_changed():
+    from ddm_amd._launch import written
+    x = torch.ones(3, requires_grad=True)
+    y = x * 2
+    z = y.pow(2).sum()                                  # keeps y
+    written(y.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        z.backward()
+    written(None)
+    with torch.inference_mode():
+        written(torch.ones(3))
