@@ -29,6 +29,11 @@ int timed(ddm_event_t begin, ddm_event_t end, hipStream_t s, F launch) {
     return end ? hip_status(hipEventRecord(reinterpret_cast<hipEvent_t>(end), s), "event record") : 0;
 }
 
+// A call that has nothing to launch: its timing events alone.
+inline int timed_nothing(ddm_event_t begin, ddm_event_t end, ddm_stream_t s) {
+    return timed(begin, end, as_hip(s), [] { return 0; });
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // 0, or DDM_E_ARG where a launch has no room for the workgroups: under 2^32 work-items.

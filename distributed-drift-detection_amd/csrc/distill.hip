@@ -344,7 +344,7 @@ extern "C" int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, in
         set_error("ddm_topk_distill: the remainder's probability is known at temperature 1 only");
         return DDM_E_ARG;
     }
-    if (n == 0) return 0;
+    if (n == 0) return timed_nothing(ev_begin, ev_end, stream);
     const int size = dtype == DDM_F32 ? 4 : 2;
     const Shape s = distill_shape(n, vectors_of(logits, ld * size, v, 16 / size));
     if (int rc = check_grid("ddm_topk_distill", n * s.parts + kQueues * kDies * s.parts, s.nt)) return rc;

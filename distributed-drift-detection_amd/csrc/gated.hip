@@ -260,7 +260,7 @@ extern "C" int ddm_gated_step(const void* x, int32_t dtype, int64_t ld_x, const 
                               float* state_out, void* out, int64_t ld_out, ddm_stream_t stream, ddm_event_t ev_begin,
                               ddm_event_t ev_end) {
     if (int rc = check("ddm_gated_step", dtype, gate_dtype, rows, d, gates, ld_x, ld_a, rows, scale, 0)) return rc;
-    if (rows == 0) return 0;
+    if (rows == 0) return timed_nothing(ev_begin, ev_end, stream);
     if (!x || !log_a || !state_out || !out || ld_out < d) {
         set_error("ddm_gated_step: invalid argument (null pointer or output stride)");
         return DDM_E_ARG;

@@ -482,7 +482,7 @@ extern "C" int ddm_token_scores(const void* logits, int32_t dtype, int64_t n, in
                                 float* top_logprob, int32_t* top_index, void* scratch, ddm_stream_t stream,
                                 ddm_event_t ev_begin, ddm_event_t ev_end) {
     if (int rc = check_rows("ddm_token_scores", dtype, n, v, ld, target_bytes, temperature, top)) return rc;
-    if (n == 0) return 0;
+    if (n == 0) return timed_nothing(ev_begin, ev_end, stream);
     const int size = dtype == DDM_F32 ? 4 : 2;
     const Shape s = shape_of(n, vectors_of(logits, ld * size, v, 16 / size), true);
     if (int rc = check_grid("ddm_token_scores", n * s.parts, s.nt)) return rc;
@@ -524,7 +524,7 @@ extern "C" int ddm_token_scores_grad(const void* logits, int32_t dtype, int64_t 
                                      const float* d_logprob, const float* d_entropy, const float* d_top, void* out,
                                      int64_t out_ld, ddm_stream_t stream, ddm_event_t ev_begin, ddm_event_t ev_end) {
     if (int rc = check_rows("ddm_token_scores_grad", dtype, n, v, ld, target_bytes, temperature, top)) return rc;
-    if (n == 0) return 0;
+    if (n == 0) return timed_nothing(ev_begin, ev_end, stream);
     if (!logits || !target || !stats || !entropy || !out || out_ld < v || (top && (!top_index || !d_top))) {
         set_error("ddm_token_scores_grad: invalid argument (null pointer or output stride)");
         return DDM_E_ARG;

@@ -376,3 +376,20 @@ def test_results_over_saved_tensors():
     with torch.inference_mode():
         y = x.clone()
         ddm_amd.token_scores_grad(y, t, r, d_logprob=d, out=y)
+
+
+def test_timers_of_calls_without_rows():
+    import ddm_amd
+    from ddm_amd.kernels import LaunchTimer
+    x, t = torch.empty(0, 100, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda")
+    r = ddm_amd.token_scores(x, t, top=2)
+    for call in (lambda timer: ddm_amd.token_scores(x, t, timer=timer),
+                 lambda timer: ddm_amd.token_scores_grad(x, t, r, timer=timer),
+                 lambda timer: ddm_amd.topk_distill(x, r.top_index, r.top_logprob, grad=True, timer=timer),
+                 lambda timer: ddm_amd.gated_step(x, x, timer=timer),
+                 lambda timer: ddm_amd.gated_scan(x, x, timer=timer),
+                 lambda timer: ddm_amd.gated_scan_grad(x, x, x, x, timer=timer)):
+        timer = LaunchTimer()
+        call(timer)
+        torch.cuda.synchronize()
+        assert 0.0 <= timer.elapsed_ms() < 1000.0
