@@ -47,7 +47,7 @@ struct SelectLds {
     uint32_t tau, n, nhits, sum[4];
 };
 
-// One wave: the k-th largest of NT keys in LDS (kKeyNegInf + 1 if fewer than k are above
+// One wave: the k-th largest (k at most 64, so at most NT) of NT keys in LDS (kKeyNegInf + 1 if fewer than k are above
 // kKeyNegInf).  Bits from the first one in which they differ, a ballot each; once exactly k
 // remain, the prefix itself will do.
 template <int NT>
@@ -66,7 +66,6 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t* keys, int k) {
         some |= __shfl_xor(some, d);
     }
     const uint32_t differ = __builtin_amdgcn_readfirstlane(all ^ some);
-    if (k > NT) return kKeyNegInf + 1;
     uint32_t prefix = __builtin_amdgcn_readfirstlane(all);
     if (differ) prefix &= ~((2u << (31 - __builtin_clz(differ))) - 1u);
     for (uint32_t bit = differ ? 1u << (31 - __builtin_clz(differ)) : 0u; bit; bit >>= 1) {
