@@ -104,8 +104,8 @@ __device__ __forceinline__ float apply(const Step& s, float h) { return s.a < 0.
 
 // ---- gates ---------------------------------------------------------------------------------------
 // 1 - e^y without cancellation, given e = e^y: for |y| <= 0.5 by (e^y - 1) / y, interpolated there in
-// seven Chebyshev points (within 1.2 half steps, rounding included), beyond as the difference, where
-// e is under 0.61.
+// seven Chebyshev points (within 1.7 * 2^-24 of the value, 1.26 units in its last place, rounding included; over
+// all float32 of [2^-6, 0.5]), beyond as the difference, where e is under 0.61.
 __device__ __forceinline__ float one_minus_exp(float y, float e) {
     float p = 1.996217616e-4f;
     p = fmaf(p, y, 1.399777364e-3f);

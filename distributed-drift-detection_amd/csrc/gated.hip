@@ -5,8 +5,8 @@ namespace ddm {
 namespace gated {
 
 // A tile's steps stay in registers, two float32 an entry; 16 rows a lane let two workgroups share a CU.
-// 65536 x 2048 bf16, "unit", 37 sequences: 228 us, 3.5 TB/s; one sequence of them 207.  What is above
-// the 165 us of the same kernel without the chain is tiles waiting for tiles.  (With the steps computed
+// 65536 x 2048 bf16, "unit", 37 sequences: 234 us, 3.4 TB/s; one sequence of them 210.  What is above
+// the 165 us of the same kernel without the chain is tiles waiting for tiles, and 4 us the look for gates over 1.  (With the steps computed
 // again after the wait, three workgroups fit a CU: "unit" 235 us, "none" no faster.)
 template <typename X, typename H, typename L, int VEC, bool OWN, int R>
 __global__ __launch_bounds__(NT, 4) void k_gated_scan(Args a) {

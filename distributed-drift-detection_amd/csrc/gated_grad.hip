@@ -7,7 +7,9 @@ namespace gated {
 // Rows in the opposite order: position p of the recurrence is row ntiles * tr - 1 - p, and a lane's
 // rows run from its last one back; bits of rows count from the first, as in the forward.  Four operands
 // a row leave room for 8 rows, and gates are computed again rather than kept, so three workgroups share
-// a CU.  65536 x 2048 bf16: 367 us, 4.4 TB/s; 16384 x 2048 bf16 with 128 gates: 94 us.
+// a CU.  65536 x 2048 bf16, one sequence: 406 us, 4.0 TB/s ("unit" in 37 sequences 418); 16384 x 2048 bf16 with 128
+// gates: 99 us.  Float32 gates of their own beside 16-bit inputs spill 12 registers: 529 us where the bytes at
+// a copy's rate take 438 (16-bit gates: 418 and 329).
 // h is of the inputs' type, half a step of which is then in the gates' gradients, or float32 (two workgroups
 // a CU, as many bytes again for a 16-bit h): the caller's choice.  16384 x 2048 bf16 with 128 gates, one
 // sequence: scan 49 -> 56 us, gradient 101 -> 123.
@@ -155,7 +157,9 @@ __global__ __launch_bounds__(NT, (std::is_same<X, H>::value ? 6 : 4)) void k_gat
     });
 }
 
-// Gates shared by more channels than a wave sums: the parts of each, in order.
+// Gates shared by more channels than a wave sums: the parts of each, in order.  An odd number of channels a gate
+// leaves every channel a part: 8192 x 1001 bf16 with one gate 344 us, gradient and sums, x 1024 48; 65536 x 1023
+// with 341 gates 404, 65536 x 1024 with 256 183.
 template <typename L>
 __global__ __launch_bounds__(256) void k_gated_sum(Args a, int64_t gates, int per) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / gates, g = i % gates;

@@ -6,14 +6,15 @@
 //   log p_i = d_i - log S,   H = log S - U / S,   rank = #{x_i > x_t or x_i = x_t, i < t}.
 // The pass is bound by reading the logits; what it computes per entry (12 vector instructions with
 // the alternatives, one of them an exponential at a quarter of the rate) takes as long as that
-// for 16-bit logits.  A row is cut into parts (shape_of), one a workgroup, so that several workgroups
+// for 16-bit logits: 8192 x 131072 are 2.05e8 instructions of a wave, 4 cycles each on 1024 units at 2.4 GHz 335
+// us, and 12 cycles more for each of 1.7e7 exponentials 80.  A row is cut into parts (shape_of), one a workgroup, so that several workgroups
 // share a CU and one's sums run behind another's loads; few rows are cut finer, until there are
 // enough workgroups for the chip.  Parts meet in a second small launch.  No atomic decides an
 // order: every sum is a fixed tree, and the alternatives are ordered by (value, index).
-// Measured: 8192 x 131072 bf16 with 32 alternatives 415 us, 5.2 TB/s and the vector unit busy all the
-// time; 4096 x 65536 bf16 without 150 us; 1000 x 50021 float32 with 5 50 us, 4.0 TB/s; one row of
+// Measured: 8192 x 131072 bf16 with 32 alternatives 417 us, 5.2 TB/s; 4096 x 65536 bf16 without 142 us; 1000 x 50021 float32 with 5 50 us, 4.0 TB/s; one row of
 // 131072 bf16 with 20 in 8 + 6.5 us, latencies of the two launches.  (A copy of 2 GB runs at
-// 4.9 TB/s, reads and writes together.)
+// 4.9 TB/s, reads and writes together.)  Rows in which more than 512 entries tie at the k-th value, a row
+// masked by the type's lowest value with fewer than k columns left among them, cost far more: see select_top.
 #include "logits.h"
 
 namespace ddm {
@@ -40,7 +41,9 @@ struct ScoreArgs {
 // lanes' bounds the k-th largest entry from below (tau).  Lanes whose largest reaches tau (little
 // more than k of them) have their entries read again, those that reach tau go to LDS and are
 // ordered by counting.  More of them than the list holds (rows of equal values) are cut exactly
-// by bisection, over entries read again each time: slow, but seldom, and bounded.
+// by bisection, over entries read again each time, up to 66 times: bounded, but slow.  64 x 32768 bf16 with 20
+// alternatives 23 us; constant rows 162; five columns above the type's lowest value 165 (above -inf 23).  4096
+// x 131072 with five above the lowest 30.8 ms instead of 0.25.
 struct SelectLds {
     uint64_t list[kListCap];
     uint32_t keys[256], hits[kListCap];
@@ -368,7 +371,7 @@ __global__ __launch_bounds__(NT) void k_score_join(ScoreArgs a) {
 // A = g_lp + sum g_top + g_H H, B = g_H: elementwise from the forward's statistics, reading and
 // writing every logit once.  The few columns with a term of their own are written again after
 // the rest of their part, in full, by one lane each.  Bound by that traffic: 4096 x 65536 bf16 in
-// 176 us, 6.1 TB/s, the logits partly still in the last cache from the forward.
+// 173 us, 6.2 TB/s, the logits partly still in the last cache from the forward.
 struct GradArgs {
     const char* x;
     int64_t n, v, ld_bytes, out_ld_bytes;

@@ -744,7 +744,7 @@ int ddm_forest_predict_dev(const ddm_predict_segment* segs_dev, const int64_t* c
 #define DDM_BF16 1
 #define DDM_F16  2
 
-/* Scores of n rows of v logits (v at most 524288; row stride ld >= v entries, any alignment)
+/* Scores of n rows (at most 33554367) of v logits (at most 524288; row stride ld >= v entries, any alignment)
  * against target[n] (target_bytes 4: int32, 8: int64), at temperature T > 0:
  *   logprob[n], entropy[n]   of softmax(x / T), float32
  *   rank[n]    entries before the target in the order (value descending, column ascending)
@@ -803,7 +803,8 @@ int ddm_topk_distill(const void* logits, int32_t dtype, int64_t n, int64_t v, in
  * NaN, in the gradient and the step as well.  out [rows][d] in x's type, the recurrence itself
  * in float32.  flags: DDM_GATED_FILL zeroes rows of no sequence, which are left alone otherwise;
  * DDM_GATED_H_F32: out (the gradient's h) is float32, so that no gate's gradient is made of a rounded
- * state.  A sequence without rows hands its state through.  Results do not depend on timing: the order of every composition is
+ * state.  A sequence without rows hands its state through.  The rows a workgroup holds (at most 4096, at most
+ * 128 from 128 channels on) lie within 2^31 bytes: a larger row stride is refused.  Results do not depend on timing: the order of every composition is
  * fixed by the sizes.  scratch: ddm_gated_scan_scratch_bytes(...) bytes, 16-byte aligned, for one
  * call at a time (NULL if 0). */
 #define DDM_GATED_NONE 0
