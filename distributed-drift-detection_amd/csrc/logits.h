@@ -13,7 +13,8 @@ namespace logits {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // exp2 of anything at or below this is 0 in float32; products e * d take d clamped here, so
-// that a masked entry (d = -inf, e = 0) adds 0 and not 0 * inf
+// that a masked entry (d = -inf, e = 0) adds 0 and not 0 * inf.  (The instruction gives 0 under 2^-126: a
+// probability that float32 holds with fewer bits counts as none.)
 constexpr float kDead = -200.0f;
 
 struct f32_t {

@@ -77,7 +77,8 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
     offsets[s+1] - 1 (None: one sequence of all rows).  state [n, d] float32: before the first rows
     (None: 0).  Rows of no sequence are zero in a new h and left alone in a given `out`, which
     may be x itself.  dtype (or out's): torch.float32 keeps h as it was computed, which gated_scan_grad makes the
-    gates' gradients of; None is x's type, and half the bytes of 16-bit inputs' h.  NaN and infinities stay within their sequence and channel."""
+    gates' gradients of; None is x's type, and half the bytes of 16-bit inputs' h.  NaN and infinities stay within their sequence and channel, where what follows an infinite state is
+    infinite or NaN (its gates' product may be 0)."""
     rows, d, gates, ld_x, ld_a = _inputs(x, log_a)
     mode = _scale(scale)
     n = _sequences(offsets, state, "state", d)
@@ -138,8 +139,8 @@ def gated_scan_grad(x, log_a, h, d_h, offsets=None, state=None, d_state=None, sc
 
 
 def gated_step(x, log_a, state=None, scale="none", out_state=None, stream=None, timer=None):
-    """One row of every sequence: row s of x [n, d] and log_a [n, gates] continues state[s] (float32,
-    None: 0).  Returns (h in x's type, the state after); out_state may be `state` itself, and lies apart
+    """One row of every sequence: row s of x [n, d] and log_a [n, gates] (as gated_scan's) continues state[s]
+    (float32, None: 0).  Returns (h in x's type, the state after); out_state may be `state` itself, and lies apart
     from x and log_a."""
     rows, d, gates, ld_x, ld_a = _inputs(x, log_a)
     mode = _scale(scale)
