@@ -2,6 +2,8 @@
 // are their own sign of having been written (unset words hold all ones), so no fence is needed.
 // Work that waits is taken by tickets, so that what it waits for already runs or starts next.
 #pragma once
+#include <stddef.h>
+
 #include "common.h"
 
 namespace ddm {
@@ -35,14 +37,16 @@ __device__ __forceinline__ void tell_gave_up() { *(volatile uint32_t*)&guard.gav
 // The current device's: a new limit (NULL: as it is), and whether a wait gave up since this was last asked (NULL: not
 // asked).  After hipDeviceSynchronize.
 [[maybe_unused]] static int use_guard(const uint32_t* looks, bool* gave_up) {
-    Guard g{};
-    if (int rc = hip_status(hipMemcpyFromSymbol(&g, HIP_SYMBOL(guard), sizeof g), "wait guard")) return rc;
+    const char* who = "wait guard";
     if (gave_up) {
-        *gave_up = *gave_up || g.gave_up;
-        g.gave_up = 0;
+        const uint32_t none = 0;
+        uint32_t one = 0;
+        if (int rc = hip_status(hipMemcpyFromSymbol(&one, HIP_SYMBOL(guard), 4, offsetof(Guard, gave_up)), who)) return rc;
+        if (one)
+            if (int rc = hip_status(hipMemcpyToSymbol(HIP_SYMBOL(guard), &none, 4, offsetof(Guard, gave_up)), who)) return rc;
+        *gave_up = *gave_up || one;
     }
-    if (looks) g.looks = *looks;
-    return hip_status(hipMemcpyToSymbol(HIP_SYMBOL(guard), &g, sizeof g), "wait guard");
+    return looks ? hip_status(hipMemcpyToSymbol(HIP_SYMBOL(guard), looks, 4, offsetof(Guard, looks)), who) : 0;
 }
 int use_guard_distill(const uint32_t* looks, bool* gave_up);
 int use_guard_gated(bool* gave_up);

@@ -71,14 +71,15 @@ def gated_scan(x, log_a, offsets=None, state=None, scale="none", out=None, strea
     h_t = exp(log_a_t) h_{t-1} + b_t, b = x ("none"), (1 - a) x ("ewma") or sqrt(1 - a^2) x ("unit").
 
     x [rows, d] float32, bfloat16 or float16; log_a [rows, gates] of x's type or float32, channel c
-    using gate c // (d // gates), at most 0 (a gate over 1 counts as NaN); rows contiguous, with a row stride (log_a's may be 0: expanded) up to 500 KB, or 15 MB from 128 channels
-    on: the rows that one workgroup holds lie within 2 GB.
+    using gate c // (d // gates), at most 0 (a gate over 1 counts as NaN); rows contiguous, with a row stride
+    (log_a's may be 0: expanded) up to 500 KB, or 15 MB from 128 channels on: the rows that one workgroup holds
+    lie within 2 GB.
     offsets int64 [n + 1] on the device, not decreasing: sequence s is rows offsets[s] ..
     offsets[s+1] - 1 (None: one sequence of all rows).  state [n, d] float32: before the first rows
     (None: 0).  Rows of no sequence are zero in a new h and left alone in a given `out`, which
     may be x itself.  dtype (or out's): torch.float32 keeps h as it was computed, which gated_scan_grad makes the
-    gates' gradients of; None is x's type, and half the bytes of 16-bit inputs' h.  NaN and infinities stay within their sequence and channel, where what follows an infinite state is
-    infinite or NaN (its gates' product may be 0)."""
+    gates' gradients of; None is x's type, and half the bytes of 16-bit inputs' h.  NaN and infinities stay within
+    their sequence and channel, where what follows an infinite state is infinite or NaN (its gates' product may be 0)."""
     rows, d, gates, ld_x, ld_a = _inputs(x, log_a)
     mode = _scale(scale)
     n = _sequences(offsets, state, "state", d)
